@@ -57,6 +57,15 @@ SIGNATURES = {
     "docc_b200_conv": (_int, [_int, _int, _int, _pi64, _pi64, _pi64, _pi64, _pi64, _i64, _i64, _vp, _vp, _vp, _vp, _int]),
     "docc_b200_attention": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _f32, _int, _vp, _pi64, _vp, _pi64, _vp, _pi64, _vp, _pi64, _int]),
     "docc_b200_layernorm": (_int, [_int, _i64, _i64, _vp, _vp, _vp, _f64, _vp, _int]),
+    "docc_b200_rmsnorm": (_int, [_int, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _f64, _vp, _vp, _int]),
+    "docc_b200_rmsnorm_q8": (_int, [_int, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _f64, _i64, _vp, _vp, _vp, _int]),
+    "docc_b200_rope": (_int, [_int, _i64, _i64, _i64, _i64, _int, _int, _vp, _pi64, _vp, _vp, _f32, _vp, _pi64, _int]),
+    "docc_b200_rope_append": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _int, _vp, _pi64, _vp, _pi64, _vp, _pi64, _vp, _vp, _f32,
+                                     _vp, _pi64, _vp, _pi64, _vp, _pi64, _i64, _i64, _vp, _int]),
+    "docc_b200_paged_attention": (_int, [_int, _i64, _i64, _i64, _i64, _f32, _f32, _i64, _vp, _pi64, _vp, _pi64, _vp, _pi64, _i64, _i64,
+                                         _vp, _i64, _i64, _vp, _vp, _pi64, _vp, _vp, _sz, _int]),
+    "docc_b200_paged_attention_workspace": (_int, [_int, _i64, _i64, _i64, _i64, ctypes.POINTER(_sz)]),
+    "docc_b200_token_logprobs": (_int, [_int, _i64, _i64, _vp, _i64, _f32, _vp, _vp, _vp, _i64, _vp, _vp, _int]),
     "docc_b200_bias_act": (_int, [_int, _i64, _i64, _vp, _f32, _vp, _int, _vp, _vp, _int]),
     "docc_b200_binary": (_int, [_int, _int, _i64, _vp, _vp, _vp, _int]),
     "docc_b200_cast": (_int, [_int, _int, _i64, _vp, _vp, _int]),

@@ -43,13 +43,28 @@ int set_error(int status, const char* fmt, ...);
     } while (0)
 
 // ---- context ----------------------------------------------------------------------------
-// Word 0 of the status block is written by kernels whose bounded waits run out; it lives in
-// mapped pinned host memory so the host can read it after a sync without a copy.
+// The status block is written by kernels whose bounded waits run out (word 0) and by kernels that meet an index in
+// device memory that points outside what the caller described (word 2); it lives in mapped pinned host memory so the
+// host can read it after a sync without a copy.
 struct DeviceStatus {
     unsigned int timeout_flag;   // != 0: a bounded device-side wait expired
     unsigned int timeout_where;  // kernel-specific location code
-    unsigned int pad[14];
+    unsigned int index_flag;     // != 0: an index read from device memory was out of range and not followed
+    unsigned int index_where;    // kIndex* code of the table it stood in
+    unsigned int pad[12];
 };
+
+enum : unsigned { kIndexPage = 1, kIndexLength = 2, kIndexSlot = 3 };
+
+#ifdef __CUDACC__
+// Every thread that meets a bad index may call this: all of them store the same kind of value, so the race is harmless.
+__device__ inline void report_bad_index(DeviceStatus* status, unsigned where) {
+    volatile unsigned int* w = &status->index_where;
+    volatile unsigned int* f = &status->index_flag;
+    *w = where;
+    *f = 1u;
+}
+#endif
 
 struct Ctx {
     int device = -1;

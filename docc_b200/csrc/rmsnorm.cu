@@ -1,0 +1,207 @@
+// RMS norm with the residual's addition, and the same norm with an 8-bit output.
+//
+//   s = x + r,  S = round(s),  y = s * rsqrt(mean(s^2) + eps) * gamma,  Y = round(y)  or  Q = e4m3(y / scale_g)
+//
+// Bandwidth bound: x and r are read once, S and Y (or Q and its scales) written once. s stays in fp32 between the sum of
+// squares and the output, so each output is rounded once.
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+#include "device_math.cuh"
+#include "ptx.cuh"
+
+namespace docc_b200 {
+namespace {
+
+constexpr int64_t kRmsMaxCols = 32768;  // the row is staged in shared memory in fp32: 128 KB of 227
+constexpr int kRmsGroup = 128;
+constexpr float kE4m3Max = 448.f;
+
+// Maximum that keeps a NaN, so that a group holding one gets a NaN scale instead of a plausible one.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float warp_max_nan(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+// y / scale with the division rounded once: a product with the rounded reciprocal would move values that lie next to the
+// middle of two codes to the other one.
+__device__ __forceinline__ uint8_t quantise(float y, float scale) {
+    return __nv_cvt_float_to_fp8(scale == 0.f ? 0.f : __fdiv_rn(y, scale), __NV_SATFINITE, __NV_E4M3);
+}
+
+struct RmsArgs {
+    int64_t rows, cols, ldx, ldr;
+    float eps;
+    const float* gamma;
+    int64_t group;  // 8-bit output: columns per scale
+};
+
+// Any width and alignment: one block per row, the row staged in shared memory.
+template <typename T, bool Q8>
+__global__ void __launch_bounds__(256) rmsnorm_row_kernel(const T* X, const T* R, T* S, T* Y, uint8_t* Q, float* scales, RmsArgs a) {
+    ptx::griddep_wait();
+    ptx::griddep_launch_dependents();
+    extern __shared__ float row_s[];
+    __shared__ float red[8];
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int cols = int(a.cols);
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* x = X + row * a.ldx;
+        const T* r = R ? R + row * a.ldr : nullptr;
+        float ss = 0.f;
+        for (int c = t; c < cols; c += 256) {
+            float v = to_float(x[c]);
+            if (r) v += to_float(r[c]);
+            row_s[c] = v;
+            if (S) S[row * a.cols + c] = from_float<T>(v);
+            ss = fmaf(v, v, ss);
+        }
+        const float rstd = rsqrtf(block_sum_f(ss, red) / float(cols) + a.eps);
+        if constexpr (!Q8) {
+            for (int c = t; c < cols; c += 256) {
+                const float y = row_s[c] * rstd;
+                Y[row * a.cols + c] = from_float<T>(a.gamma ? y * a.gamma[c] : y);
+            }
+        } else {
+            // a group per warp in turn; a whole-row group is the one group of warp 0..7 together
+            const int64_t groups = (a.cols + a.group - 1) / a.group;
+            if (a.group >= a.cols) {
+                float m = 0.f;
+                for (int c = t; c < cols; c += 256) {
+                    const float y = a.gamma ? row_s[c] * rstd * a.gamma[c] : row_s[c] * rstd;
+                    row_s[c] = y;
+                    m = max_nan(m, fabsf(y));
+                }
+                m = warp_max_nan(m);
+                __syncthreads();
+                if (lane == 0) red[warp] = m;
+                __syncthreads();
+                m = red[0];
+                for (int w = 1; w < 8; w++) m = max_nan(m, red[w]);
+                const float scale = __fdiv_rn(m, kE4m3Max);
+                for (int c = t; c < cols; c += 256) Q[row * a.cols + c] = quantise(row_s[c], scale);
+                if (t == 0) scales[row] = scale;
+            } else {
+                for (int g = warp; g < groups; g += 8) {
+                    const int c0 = int(g * a.group), c1 = int(c0 + a.group < a.cols ? c0 + a.group : a.cols);
+                    float y[kRmsGroup / 32], m = 0.f;
+#pragma unroll
+                    for (int i = 0; i < kRmsGroup / 32; i++) {
+                        const int c = c0 + lane + 32 * i;
+                        y[i] = 0.f;
+                        if (c < c1) y[i] = a.gamma ? row_s[c] * rstd * a.gamma[c] : row_s[c] * rstd;
+                        m = max_nan(m, fabsf(y[i]));
+                    }
+                    const float scale = __fdiv_rn(warp_max_nan(m), kE4m3Max);
+#pragma unroll
+                    for (int i = 0; i < kRmsGroup / 32; i++) {
+                        const int c = c0 + lane + 32 * i;
+                        if (c < c1) Q[row * a.cols + c] = quantise(y[i], scale);
+                    }
+                    if (lane == 0) scales[row * groups + g] = scale;
+                }
+            }
+        }
+        __syncthreads();  // row_s and red are reused by the next row
+    }
+}
+
+template <typename T, bool Q8>
+int rms_device(Ctx* ctx, const RmsArgs& a, const void* X, const void* R, void* S, void* Y, void* Q, void* scales) {
+    const size_t smem = size_t(a.cols) * 4;
+    auto kernel = rmsnorm_row_kernel<T, Q8>;
+    if (smem > 48 * 1024) DOCC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+    const int64_t cap = int64_t(ctx->sm_count) * 8;
+    const int grid = int(a.rows < cap ? a.rows : cap);
+    DOCC_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(256), smem, ctx->stream, static_cast<const T*>(X), static_cast<const T*>(R),
+                             static_cast<T*>(S), static_cast<T*>(Y), static_cast<uint8_t*>(Q), static_cast<float*>(scales), a));
+    return after_launch(ctx, "rmsnorm_row_kernel");
+}
+
+int rms_any(Ctx* ctx, int prec, const RmsArgs& a, const void* X, const void* R, void* S, void* Y, void* Q, void* scales) {
+    const bool q8 = Q != nullptr;
+    switch (prec) {
+        case DOCC_B200_PREC_S:
+            return q8 ? rms_device<float, true>(ctx, a, X, R, S, Y, Q, scales) : rms_device<float, false>(ctx, a, X, R, S, Y, Q, scales);
+        case DOCC_B200_PREC_H:
+            return q8 ? rms_device<__half, true>(ctx, a, X, R, S, Y, Q, scales) : rms_device<__half, false>(ctx, a, X, R, S, Y, Q, scales);
+        default:
+            return q8 ? rms_device<__nv_bfloat16, true>(ctx, a, X, R, S, Y, Q, scales)
+                      : rms_device<__nv_bfloat16, false>(ctx, a, X, R, S, Y, Q, scales);
+    }
+}
+
+int rms_checked(const char* what, int prec, const RmsArgs& a, const void* X, const void* R, void* S, void* Y, void* Q, void* scales,
+                int flags) {
+    DOCC_REQUIRE(prec == DOCC_B200_PREC_S || prec == DOCC_B200_PREC_B || prec == DOCC_B200_PREC_H,
+                 "%s: precision %d not supported (use 's', 'b' or 'h')", what, prec);
+    DOCC_REQUIRE(a.rows >= 0 && a.cols >= 0, "%s: negative extent", what);
+    DOCC_REQUIRE(a.eps >= 0.f, "%s: eps must not be negative", what);
+    Ctx* ctx;
+    DOCC_TRY(get_ctx(&ctx));
+    if (a.rows == 0 || a.cols == 0) return DOCC_B200_OK;
+    DOCC_REQUIRE(X && (Y || (Q && scales)), "%s: NULL data pointer", what);
+    DOCC_REQUIRE(a.ldx >= a.cols && (!R || a.ldr >= a.cols), "%s: row stride below cols", what);
+    if (a.cols > kRmsMaxCols) return set_error(DOCC_B200_ERR_UNSUPPORTED, "%s: cols %lld > %lld", what, (long long)a.cols, (long long)kRmsMaxCols);
+    if (!(flags & DOCC_B200_FLAG_HOST_PTRS)) return rms_any(ctx, prec, a, X, R, S, Y, Q, scales);
+
+    DOCC_REQUIRE(a.ldx == a.cols && (!R || a.ldr == a.cols), "%s: host pointers require contiguous rows", what);
+    const size_t n = size_t(a.rows) * size_t(a.cols), es = prec_size(prec);
+    const size_t n_scales = Q ? size_t(a.rows) * size_t(ceil_div(a.cols, a.group)) * 4 : 0;
+    TempBuffers tmp;
+    void *dX, *dR = nullptr, *dG = nullptr, *dS = nullptr, *dY = nullptr, *dQ = nullptr, *dScales = nullptr;
+    RmsArgs d = a;
+    DOCC_TRY(tmp.alloc(&dX, n * es));
+    DOCC_CUDA_TRY(cudaMemcpyAsync(dX, X, n * es, cudaMemcpyHostToDevice, ctx->stream));
+    if (R) {
+        DOCC_TRY(tmp.alloc(&dR, n * es));
+        DOCC_CUDA_TRY(cudaMemcpyAsync(dR, R, n * es, cudaMemcpyHostToDevice, ctx->stream));
+    }
+    if (a.gamma) {
+        DOCC_TRY(tmp.alloc(&dG, size_t(a.cols) * 4));
+        DOCC_CUDA_TRY(cudaMemcpyAsync(dG, a.gamma, size_t(a.cols) * 4, cudaMemcpyHostToDevice, ctx->stream));
+        d.gamma = static_cast<const float*>(dG);
+    }
+    if (S) DOCC_TRY(tmp.alloc(&dS, n * es));
+    if (Q) {
+        DOCC_TRY(tmp.alloc(&dQ, n));
+        DOCC_TRY(tmp.alloc(&dScales, n_scales));
+    } else {
+        DOCC_TRY(tmp.alloc(&dY, n * es));
+    }
+    DOCC_TRY(rms_any(ctx, prec, d, dX, dR, dS, dY, dQ, dScales));
+    if (S) DOCC_CUDA_TRY(cudaMemcpyAsync(S, dS, n * es, cudaMemcpyDeviceToHost, ctx->stream));
+    if (Q) {
+        DOCC_CUDA_TRY(cudaMemcpyAsync(Q, dQ, n, cudaMemcpyDeviceToHost, ctx->stream));
+        DOCC_CUDA_TRY(cudaMemcpyAsync(scales, dScales, n_scales, cudaMemcpyDeviceToHost, ctx->stream));
+    } else {
+        DOCC_CUDA_TRY(cudaMemcpyAsync(Y, dY, n * es, cudaMemcpyDeviceToHost, ctx->stream));
+    }
+    DOCC_CUDA_TRY(cudaStreamSynchronize(ctx->stream));
+    return DOCC_B200_OK;
+}
+
+}  // namespace
+}  // namespace docc_b200
+
+using namespace docc_b200;
+
+extern "C" int docc_b200_rmsnorm(int prec, int64_t rows, int64_t cols, const void* X, int64_t ldx, const void* residual, int64_t ldr,
+                                 const void* gamma, double eps, void* S, void* Y, int flags) {
+    const RmsArgs a{rows, cols, ldx, ldr, float(eps), static_cast<const float*>(gamma), cols};
+    DOCC_REQUIRE(rows * cols == 0 || Y, "rmsnorm: NULL data pointer");
+    return rms_checked("rmsnorm", prec, a, X, residual, S, Y, nullptr, nullptr, flags);
+}
+
+extern "C" int docc_b200_rmsnorm_q8(int prec, int64_t rows, int64_t cols, const void* X, int64_t ldx, const void* residual, int64_t ldr,
+                                    const void* gamma, double eps, int64_t group, void* S, void* Q, void* scales, int flags) {
+    DOCC_REQUIRE(group == 0 || group == kRmsGroup, "rmsnorm_q8: group %lld (use 0 for whole rows or %d)", (long long)group, kRmsGroup);
+    const RmsArgs a{rows, cols, ldx, ldr, float(eps), static_cast<const float*>(gamma), group ? group : cols};
+    DOCC_REQUIRE(rows * cols == 0 || (Q && scales), "rmsnorm_q8: NULL data pointer");
+    return rms_checked("rmsnorm_q8", prec, a, X, residual, S, nullptr, Q, scales, flags);
+}

@@ -386,6 +386,13 @@ int docc_b200_sync(void) {
         c->status_host->timeout_where = 0;
         return set_error(DOCC_B200_ERR_DEVICE_TIMEOUT, "a bounded device-side wait ran out (location code %u)", where);
     }
+    if (c->status_host->index_flag) {
+        const unsigned where = c->status_host->index_where;
+        c->status_host->index_flag = 0;
+        c->status_host->index_where = 0;
+        return set_error(DOCC_B200_ERR_BAD_INDEX, "a kernel met %s out of range and did not follow it",
+                         where == kIndexPage ? "a page number" : where == kIndexLength ? "a sequence length" : "a cache slot");
+    }
     return DOCC_B200_OK;
 }
 
@@ -398,6 +405,7 @@ const char* docc_b200_strerror(int status) {
         case DOCC_B200_ERR_OOM: return "out of memory";
         case DOCC_B200_ERR_NO_DEVICE: return "no usable sm_100 device";
         case DOCC_B200_ERR_DEVICE_TIMEOUT: return "device-side wait timed out";
+        case DOCC_B200_ERR_BAD_INDEX: return "index in device memory out of range";
         default: return "unknown status";
     }
 }

@@ -338,6 +338,287 @@ def layernorm(X, gamma=None, beta=None, eps=1e-5, flags=0):
     return Y
 
 
+# ---- the decoder step: RMS norm, rotary positions and the paged cache, attention over it, log-probabilities -----------------------
+def _side(*xs):
+    """``_kind`` without its demand for contiguity, for entries that take strides: flags, after checking that all arrays live on the
+    same side and, for torch tensors, on the device that the calling thread's launches go to."""
+    xs = [x for x in xs if x is not None]
+    device = [_is_torch(x) or isinstance(x, DeviceArray) for x in xs]
+    if not any(device):
+        for x in xs:
+            if not x.flags["C_CONTIGUOUS"]:
+                raise ValueError("arrays must be C-contiguous")
+        return FLAG_HOST_PTRS
+    if not all(device):
+        raise TypeError("mix of host arrays and device tensors")
+    current = None
+    for x in xs:
+        if not _is_torch(x):
+            continue
+        if not x.is_cuda:
+            raise TypeError("torch tensors must live on a CUDA device (pass numpy arrays for host data)")
+        if current is None:
+            import torch
+
+            current = torch.cuda.current_device()
+        if x.get_device() != current:
+            raise ValueError(f"tensor on cuda:{x.get_device()} while the calling thread's device is cuda:{current}")
+    return 0
+
+
+def _strides(x):
+    """Element strides of all dimensions."""
+    if _is_torch(x):
+        return x.stride()
+    out, n = [], 1
+    for s in reversed(x.shape):
+        out.append(n)
+        n *= int(s)
+    return tuple(reversed(out))
+
+
+def _heads_strides(x, name, written=False):
+    """The strides array of a tensor whose last dimension is contiguous, or NULL if all of it is. One that is written may not be
+    a broadcast view, whose elements share memory."""
+    if not _is_torch(x) or x.is_contiguous():
+        return None
+    s = x.stride()
+    if written and any(v == 0 and n > 1 for v, n in zip(s, x.shape)):
+        raise ValueError(f"{name}: a broadcast view cannot be written")
+    if s[-1] != 1 and x.shape[-1] > 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+    if any(v < 0 for v in s):
+        raise ValueError(f"{name}: negative strides")
+    return _arr(s[:-1])
+
+
+def _rows_of(x, name):
+    """(rows, cols, row stride) of a tensor seen as rows over its last dimension; the leading dimensions must be one strided run."""
+    cols = int(x.shape[-1])
+    rows = 1
+    for s in x.shape[:-1]:
+        rows *= int(s)
+    if not _is_torch(x) or x.is_contiguous():
+        return rows, cols, cols
+    s = x.stride()
+    run = s[-2] if x.ndim > 1 else cols
+    step = run
+    for d in range(x.ndim - 2, -1, -1):
+        if x.shape[d] != 1 and s[d] != step:
+            raise ValueError(f"{name}: the leading dimensions are not one run of rows")
+        step *= x.shape[d]
+    if (s[-1] != 1 and cols > 1) or (run < cols and rows > 1):
+        raise ValueError(f"{name}: rows must be contiguous and must not overlap")
+    return rows, cols, max(run, cols)
+
+
+def _want(x, dtype, name, shape=None):
+    got = str(x.dtype).replace("torch.", "") if _is_torch(x) else np.dtype(x.dtype).name
+    if got != dtype:
+        raise TypeError(f"{name} must be {dtype}, not {got}")
+    if shape is not None and tuple(x.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(x.shape)}")
+    if _is_torch(x) and not x.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _like(x, name):
+    """The element type ``name`` in the library ``x`` comes from."""
+    if _is_torch(x):
+        import torch
+
+        return getattr(torch, name)
+    return np.dtype(name)
+
+
+def _rms_inputs(X, gamma, residual, flags):
+    flags |= _side(X, gamma, residual)
+    if X.ndim == 0:
+        raise ValueError("rmsnorm: a scalar has no rows")
+    rows, cols, ldx = _rows_of(X, "rmsnorm")
+    ldr = 0
+    if gamma is not None:
+        _want(gamma, "float32", "rmsnorm: gamma", (cols,))
+    if residual is not None:
+        if tuple(residual.shape) != tuple(X.shape) or _prec(residual) != _prec(X):
+            raise ValueError("rmsnorm: the residual must have the shape and type of the input")
+        ldr = _rows_of(residual, "rmsnorm: residual")[2]
+    return rows, cols, ldx, ldr, flags
+
+
+def rmsnorm(X, gamma=None, residual=None, eps=1e-6, flags=0):
+    """``Y = s / sqrt(mean(s^2) + eps) * gamma`` over the last dimension, ``s = X + residual``. Returns Y, or with a residual
+    ``(Y, S)``: S is s in the input's type, the residual of what follows. ``gamma`` is float32."""
+    rows, cols, ldx, ldr, flags = _rms_inputs(X, gamma, residual, flags)
+    Y = _empty(X, X.shape)
+    S = _empty(X, X.shape) if residual is not None else None
+    call("docc_b200_rmsnorm", _prec(X), rows, cols, _ptr(X), ldx, _ptr(residual), ldr, _ptr(gamma), float(eps), _ptr(S), _ptr(Y), flags)
+    return Y if residual is None else (Y, S)
+
+
+def rmsnorm_quant(X, gamma=None, residual=None, eps=1e-6, group=0, flags=0):
+    """The norm of ``rmsnorm`` with an 8-bit output: ``(Q, scales)``, or ``(Q, scales, S)`` with a residual. Q holds e4m3 values
+    (``torch.float8_e4m3fn``; their codes as uint8 for other arrays) and ``Q * scales`` stands for the norm, with one float32 scale
+    per ``group`` of 128 columns or, with group 0, per row: scales have shape ``X.shape[:-1] + (groups,)``."""
+    rows, cols, ldx, ldr, flags = _rms_inputs(X, gamma, residual, flags)
+    if group not in (0, 128):
+        raise ValueError("rmsnorm_quant: group must be 0 (whole rows) or 128")
+    lead = tuple(X.shape[:-1])
+    Q = _empty(X, X.shape, _like(X, "float8_e4m3fn" if _is_torch(X) else "uint8"))
+    scales = _empty(X, lead + (1 if group == 0 else -(-cols // group),), _like(X, "float32"))
+    S = _empty(X, X.shape) if residual is not None else None
+    call("docc_b200_rmsnorm_q8", _prec(X), rows, cols, _ptr(X), ldx, _ptr(residual), ldr, _ptr(gamma), float(eps), int(group), _ptr(S),
+         _ptr(Q), _ptr(scales), flags)
+    return (Q, scales) if residual is None else (Q, scales, S)
+
+
+def rope_frequencies(rotary_dim, base=10000.0, scaling="none", factor=1.0, original_length=None, beta_fast=32.0, beta_slow=1.0):
+    """``(inv_freq, mscale)`` for ``rope``: radians per position of each pair as a float64 numpy array (``base ** (-2i / rotary_dim)``,
+    to be moved to the device once), and the factor of cosine and sine. ``scaling`` stretches a context trained at
+    ``original_length`` by ``factor``: ``"linear"`` divides every frequency; ``"ntk"`` raises the base so that the slowest pair is
+    divided by ``factor`` and the fastest kept; ``"yarn"`` divides the pairs that turn less than ``beta_slow`` times within
+    ``original_length``, keeps those that turn more than ``beta_fast`` times, blends between, and sets
+    ``mscale = 0.1 ln(factor) + 1``."""
+    rotary_dim = int(rotary_dim)
+    if rotary_dim < 0 or rotary_dim % 2:
+        raise ValueError("rope_frequencies: rotary_dim must be even")
+    if not base > 1.0 or not factor >= 1.0:
+        raise ValueError("rope_frequencies: base must be above 1 and factor at least 1")
+    i = np.arange(rotary_dim // 2, dtype=np.float64)
+    freq = float(base) ** (-2.0 * i / max(rotary_dim, 1))
+    if scaling == "none":
+        return freq, 1.0
+    if scaling == "linear":
+        return freq / factor, 1.0
+    if scaling == "ntk":
+        if rotary_dim <= 2:
+            raise ValueError("rope_frequencies: 'ntk' needs more than one pair")
+        return (base * factor ** (rotary_dim / (rotary_dim - 2.0))) ** (-2.0 * i / rotary_dim), 1.0
+    if scaling != "yarn":
+        raise ValueError(f"rope_frequencies: unknown scaling {scaling!r}")
+    if original_length is None or not beta_fast > beta_slow:
+        raise ValueError("rope_frequencies: 'yarn' needs original_length, and beta_fast above beta_slow")
+    pair_of = lambda turns: rotary_dim * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(base))
+    low, high = max(math.floor(pair_of(beta_fast)), 0), min(math.ceil(pair_of(beta_slow)), rotary_dim - 1)
+    stretched = np.clip((i - low) / max(high - low, 0.001), 0.0, 1.0)
+    return freq / factor * stretched + freq * (1.0 - stretched), 0.1 * math.log(factor) + 1.0
+
+
+def rope(X, positions, inv_freq, interleaved=False, mscale=1.0, inverse=False, out=None, flags=0):
+    """Rotary positions on X [tokens, heads, D] (``docc_b200_rope``): ``positions`` int64 [tokens], ``inv_freq`` float64
+    [rotary_dim / 2] on the side of X (``rope_frequencies``). ``inverse`` applies the transpose, which is the gradient. ``out`` may be
+    X itself."""
+    flags |= _side(X, positions, inv_freq, out)
+    if X.ndim != 3:
+        raise ValueError("rope: X must be [tokens, heads, D]")
+    T, H, D = X.shape
+    _want(positions, "int64", "rope: positions", (T,))
+    _want(inv_freq, "float64", "rope: inv_freq")
+    if inv_freq.ndim != 1 or 2 * inv_freq.shape[0] > D:
+        raise ValueError("rope: inv_freq must hold one frequency per pair, at most D / 2")
+    if out is None:
+        out = _empty(X, X.shape)
+    elif tuple(out.shape) != tuple(X.shape) or _prec(out) != _prec(X):
+        raise ValueError("rope: out must have the shape and type of X")
+    xs, ys = _heads_strides(X, "rope: X"), _heads_strides(out, "rope: out", True)
+    call("docc_b200_rope", _prec(X), T, H, D, 2 * inv_freq.shape[0], int(bool(interleaved)), int(bool(inverse)), _ptr(X), xs,
+         _ptr(positions), _ptr(inv_freq), float(mscale), _ptr(out), ys, flags)
+    return out
+
+
+def _cache(k_cache, v_cache, Hkv, D, prec, name):
+    """(pages, page_size, strides of K, strides of V) of a cache [pages, Hkv, page_size, D] (views of other layouts included)."""
+    for c in (k_cache, v_cache):
+        if c.ndim != 4 or c.shape[1] != Hkv or c.shape[3] != D or _prec(c) != prec:
+            raise ValueError(f"{name}: caches must be [pages, {Hkv}, page_size, {D}] of the type of the query")
+    if tuple(k_cache.shape) != tuple(v_cache.shape):
+        raise ValueError(f"{name}: the two caches differ in shape")
+    return (int(k_cache.shape[0]), int(k_cache.shape[2]), _heads_strides(k_cache, f"{name}: k_cache", True),
+            _heads_strides(v_cache, f"{name}: v_cache", True))
+
+
+def rope_append(q, k, v, positions, inv_freq, k_cache, v_cache, slots, interleaved=False, mscale=1.0, out=None, flags=0):
+    """Rotates q [tokens, Hq, D] and k [tokens, Hkv, D] and writes the rotated k and v into the paged cache
+    [pages, Hkv, page_size, D] at ``slots`` (int64 [tokens]: page * page_size + place; negative: not written). Returns the rotated q
+    (``out``, which may be q itself). Device tensors only; the slots of one call must differ."""
+    if _side(q, k, v, positions, inv_freq, k_cache, v_cache, slots, out):
+        raise TypeError("rope_append: the cache lives on the device; host arrays are not taken")
+    if q.ndim != 3 or k.ndim != 3 or tuple(k.shape) != tuple(v.shape) or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+        raise ValueError("rope_append: q must be [tokens, Hq, D], k and v [tokens, Hkv, D]")
+    T, Hq, D = q.shape
+    Hkv, prec = k.shape[1], _prec(q)
+    if _prec(k) != prec or _prec(v) != prec:
+        raise TypeError("rope_append: q, k and v differ in type")
+    _want(positions, "int64", "rope_append: positions", (T,))
+    _want(slots, "int64", "rope_append: slots", (T,))
+    _want(inv_freq, "float64", "rope_append: inv_freq")
+    if inv_freq.ndim != 1 or 2 * inv_freq.shape[0] > D:
+        raise ValueError("rope_append: inv_freq must hold one frequency per pair, at most D / 2")
+    pages, page_size, ks, vs = _cache(k_cache, v_cache, Hkv, D, prec, "rope_append")
+    if out is None:
+        out = _empty(q, q.shape)
+    elif tuple(out.shape) != tuple(q.shape) or _prec(out) != prec:
+        raise ValueError("rope_append: out must have the shape and type of q")
+    call("docc_b200_rope_append", prec, T, Hq, Hkv, D, 2 * inv_freq.shape[0], int(bool(interleaved)), _ptr(q),
+         _heads_strides(q, "rope_append: q"), _ptr(k), _heads_strides(k, "rope_append: k"), _ptr(v), _heads_strides(v, "rope_append: v"),
+         _ptr(positions), _ptr(inv_freq), float(mscale), _ptr(out), _heads_strides(out, "rope_append: out", True), _ptr(k_cache), ks,
+         _ptr(v_cache), vs, pages, page_size, _ptr(slots), flags)
+    return out
+
+
+def paged_attention(q, k_cache, v_cache, page_table, lengths, scale=None, softcap=0.0, window=0, return_lse=False, out=None, flags=0):
+    """Attention of one new token per sequence, q [B, Hq, D], over a paged cache [pages, Hkv, page_size, D]; the cache must already
+    hold the new token (``rope_append``). ``page_table`` int32 [B, max_pages], ``lengths`` int32 [B]: token j of sequence b is at place
+    ``j % page_size`` of page ``page_table[b, j // page_size]``. ``window`` > 0 keeps the last ``window`` tokens, ``softcap`` > 0 caps
+    the scores (``docc_b200_paged_attention``). Returns the output [B, Hq, D], with ``return_lse`` also the float32 [B, Hq]
+    logarithm of the softmax's denominator. Sequences of length 0 give zeros and -inf. Device tensors only.
+
+    With torch tensors the scratch comes from torch's allocator, so a captured graph owns the scratch it replays with."""
+    if _side(q, k_cache, v_cache, page_table, lengths, out):
+        raise TypeError("paged_attention: the cache lives on the device; host arrays are not taken")
+    if q.ndim != 3:
+        raise ValueError("paged_attention: q must be [B, Hq, D]")
+    B, Hq, D = q.shape
+    Hkv, prec = k_cache.shape[1], _prec(q)
+    pages, page_size, ks, vs = _cache(k_cache, v_cache, Hkv, D, prec, "paged_attention")
+    if Hkv == 0 or Hq % Hkv:
+        raise ValueError(f"paged_attention: {Hq} query heads are not a multiple of {Hkv} key-value heads")
+    _want(lengths, "int32", "paged_attention: lengths", (B,))
+    if page_table.ndim != 2:
+        raise ValueError("paged_attention: page_table must be [B, max_pages]")
+    _want(page_table, "int32", "paged_attention: page_table", (B, page_table.shape[1]))
+    if out is None:
+        out = _empty(q, q.shape)
+    elif tuple(out.shape) != tuple(q.shape) or _prec(out) != prec:
+        raise ValueError("paged_attention: out must have the shape and type of q")
+    lse = _empty(q, (B, Hq), _like(q, "float32")) if return_lse else None
+    bytes_ = _lib._sz()
+    call("docc_b200_paged_attention_workspace", prec, B, Hq, Hkv, D, ctypes.byref(bytes_))
+    work = _empty(q, (bytes_.value,), _like(q, "uint8")) if bytes_.value and _is_torch(q) else None
+    call("docc_b200_paged_attention", prec, B, Hq, Hkv, D, 1.0 / math.sqrt(max(D, 1)) if scale is None else float(scale), float(softcap),
+         int(window), _ptr(q), _heads_strides(q, "paged_attention: q"), _ptr(k_cache), ks, _ptr(v_cache), vs, pages, page_size,
+         _ptr(page_table), page_table.shape[1], page_table.shape[1], _ptr(lengths), _ptr(out),
+         _heads_strides(out, "paged_attention: out", True), _ptr(lse), _ptr(work), bytes_.value if work is not None else 0, flags)
+    return (out, lse) if return_lse else out
+
+
+def token_logprobs(logits, ids, k=0, scale=1.0, flags=0):
+    """``(logp, entropy, top_ids, top_logp)`` of logits [rows, vocab] under ``softmax(scale * logits)``: the log-probability of token
+    ``ids[row]`` (int64; an id outside the vocabulary gives NaN), the distribution's entropy, and the ``k`` <= 32 most likely tokens
+    with their log-probabilities (ties to the lowest index). float32, indices int64; [rows, k] for the last two."""
+    flags |= _side(logits, ids)
+    if logits.ndim != 2:
+        raise ValueError("token_logprobs: logits must be [rows, vocab]")
+    rows, vocab, ldx = _rows_of(logits, "token_logprobs")
+    _want(ids, "int64", "token_logprobs: ids", (rows,))
+    f32, i64 = _like(logits, "float32"), _like(logits, "int64")
+    logp, entropy = _empty(logits, (rows,), f32), _empty(logits, (rows,), f32)
+    top_ids, top_logp = _empty(logits, (rows, k), i64), _empty(logits, (rows, k), f32)
+    call("docc_b200_token_logprobs", _prec(logits), rows, vocab, _ptr(logits), ldx, float(scale), _ptr(ids), _ptr(logp), _ptr(entropy),
+         int(k), _ptr(top_ids), _ptr(top_logp), flags)
+    return logp, entropy, top_ids, top_logp
+
+
 def bias_act(X, scale=1.0, bias=None, act=ACT_NONE, residual=None, flags=0):
     flags |= _kind(X, bias, residual)
     cols = X.shape[-1] if X.ndim else 1

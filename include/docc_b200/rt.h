@@ -45,7 +45,9 @@ enum {
     DOCC_B200_ERR_CUDA = 3,          /* a CUDA runtime/driver call failed */
     DOCC_B200_ERR_OOM = 4,           /* device or pinned-host allocation failed / limit hit */
     DOCC_B200_ERR_NO_DEVICE = 5,     /* no usable sm_100 device */
-    DOCC_B200_ERR_DEVICE_TIMEOUT = 6 /* a bounded device-side wait ran out (status word set by the kernel) */
+    DOCC_B200_ERR_DEVICE_TIMEOUT = 6, /* a bounded device-side wait ran out (status word set by the kernel) */
+    DOCC_B200_ERR_BAD_INDEX = 7 /* a page number, length or slot in device memory was out of range; it was not followed
+                                   (status word set by the kernel, returned once by docc_b200_sync) */
 };
 
 /* ---- precision codes (BLAS_Precision, blas_node.h:49-55; 'b' is an extension) */
@@ -248,6 +250,82 @@ int docc_b200_attention(int prec, int64_t B, int64_t H, int64_t Sq, int64_t Skv,
 int docc_b200_layernorm(int prec, int64_t rows, int64_t cols,
                         const void* X, const void* gamma, const void* beta,
                         double eps, void* Y, int flags);
+
+/* ---- RMS norm ----------------------------------------------------------------------
+ * s = X + residual (fp32; residual may be NULL), S = s rounded to prec (S may be NULL without a
+ * residual), Y = s / sqrt(mean(s^2) + eps) * gamma over the last dimension. The norm takes the
+ * unrounded s, so each output is rounded once. gamma is fp32 and may be NULL. prec 's', 'b' or
+ * 'h'. X and residual have row strides ldx, ldr >= cols; S and Y are contiguous. S may be the
+ * residual's own buffer (ldr == cols) and Y the input's (ldx == cols). cols <= 32768.
+ * docc has no such node; it stands beside the LayerNorm above. */
+int docc_b200_rmsnorm(int prec, int64_t rows, int64_t cols, const void* X, int64_t ldx,
+                      const void* residual, int64_t ldr, const void* gamma, double eps,
+                      void* S, void* Y, int flags);
+/* The same norm y with an 8-bit output: columns are taken in groups of `group` (128, or 0 for the
+ * whole row; the last group may be shorter), scale = max|y| / 448 of the group in fp32, and
+ * Q = e4m3(y / scale), rounded to nearest even. A group of zeros has scale 0 and Q 0; a group that
+ * holds a NaN has scale NaN. Q: rows x cols bytes; scales: rows x ceil(cols / group) fp32. */
+int docc_b200_rmsnorm_q8(int prec, int64_t rows, int64_t cols, const void* X, int64_t ldx,
+                         const void* residual, int64_t ldr, const void* gamma, double eps,
+                         int64_t group, void* S, void* Q, void* scales, int flags);
+
+/* ---- rotary positions ---------------------------------------------------------------
+ * Y[t,h] = X[t,h] with its first rotary_dim elements rotated in pairs by a = positions[t] *
+ * inv_freq[i], i < rotary_dim / 2: (u, v) -> mscale * (u cos a - v sin a, v cos a + u sin a). Pairs
+ * are (i, i + rotary_dim / 2), or (2i, 2i + 1) with interleaved != 0. Elements from rotary_dim on
+ * are copied. The angle is formed and reduced in fp64. inverse != 0 rotates by -a, which is the
+ * transpose of the forward map and hence its gradient. Element (t,h,d) is at base + t*st + h*sh + d;
+ * NULL strides mean contiguous [tokens, heads, D]. Y may be X itself (with the same strides).
+ * positions: int64 on the side of the data, inv_freq: fp64 likewise. prec 's', 'b' or 'h'. */
+int docc_b200_rope(int prec, int64_t tokens, int64_t heads, int64_t D, int64_t rotary_dim,
+                   int interleaved, int inverse, const void* X, const int64_t* x_strides /*[st,sh] or NULL*/,
+                   const int64_t* positions, const double* inv_freq, float mscale,
+                   void* Y, const int64_t* y_strides, int flags);
+/* One step's tokens enter a paged key-value cache: Qout = rope(Q), and for every token with
+ * 0 <= slots[t] < num_pages * page_size the rotated K[t] and V[t] are written at place
+ * slots[t] % page_size of page slots[t] / page_size. A negative slot writes nothing (a padding
+ * token); one past the end writes nothing and is reported by docc_b200_sync as
+ * DOCC_B200_ERR_BAD_INDEX. Slots of one call must differ. Cache element (page, h, place, d) is at
+ * base + page*sp + h*sh + place*ss + d; NULL strides mean contiguous [num_pages, Hkv, page_size, D].
+ * Device pointers only: the cache lives on the device. */
+int docc_b200_rope_append(int prec, int64_t tokens, int64_t Hq, int64_t Hkv, int64_t D, int64_t rotary_dim, int interleaved,
+                          const void* Q, const int64_t* q_strides, const void* K, const int64_t* k_strides,
+                          const void* V, const int64_t* v_strides, const int64_t* positions, const double* inv_freq, float mscale,
+                          void* Qout, const int64_t* qo_strides,
+                          void* Kcache, const int64_t* kc_strides /*[sp,sh,ss] or NULL*/, void* Vcache, const int64_t* vc_strides,
+                          int64_t num_pages, int64_t page_size, const int64_t* slots, int flags);
+
+/* ---- attention of one new token over a paged cache -------------------------------------
+ * O[b,h] = sum_j p_j V_j, p = softmax_j(s_j), s_j = scale * Q[b,h] . K_j over the cached tokens
+ * max(0, n - window) <= j < n of sequence b, n = lengths[b] (window 0: all). softcap c > 0 replaces
+ * s by c * tanh(s / c). Token j lies at place j % page_size of page page_table[b * table_stride +
+ * j / page_size]; query head h reads key-value head h / (Hq / Hkv). lse (fp32 [B, Hq], may be NULL)
+ * receives log sum_j exp(s_j). A sequence without visible tokens gives O = 0 and lse = -inf.
+ * lengths and page_table are int32 in device memory, read when the kernel runs. A length outside
+ * [0, max_pages * page_size] is clamped and the tokens of a page number outside [0, num_pages) are
+ * left out; both are reported by docc_b200_sync as DOCC_B200_ERR_BAD_INDEX.
+ * Strides: Q, O [sb,sh]; caches [sp,sh,ss] as above; NULL = contiguous. D <= 256, prec 's', 'b', 'h'.
+ * The scratch holds partial results of sequences that several blocks share. workspace == NULL uses
+ * the calling thread's own (ordered on its stream); a caller that captures graphs which may run at
+ * the same time passes one per graph, of docc_b200_paged_attention_workspace() bytes. Device
+ * pointers only. */
+int docc_b200_paged_attention(int prec, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, float scale, float softcap, int64_t window,
+                              const void* Q, const int64_t* q_strides /*[sb,sh] or NULL*/,
+                              const void* Kcache, const int64_t* kc_strides, const void* Vcache, const int64_t* vc_strides,
+                              int64_t num_pages, int64_t page_size,
+                              const int32_t* page_table, int64_t max_pages, int64_t table_stride, const int32_t* lengths,
+                              void* O, const int64_t* o_strides, void* lse, void* workspace, size_t workspace_bytes, int flags);
+int docc_b200_paged_attention_workspace(int prec, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, size_t* bytes);
+
+/* ---- log-probabilities of given tokens ---------------------------------------------------
+ * Per row of logits X [rows x vocab] (row stride ldx): z = scale * x, lse = log sum exp z,
+ * logp = z[ids[row]] - lse, entropy = -sum p log p with p = exp(z - lse), and the k largest logits
+ * (0 <= k <= 32, ties to the lowest index, NaN counts as largest): their indices and z - lse, in
+ * descending order. One pass over X. An id outside [0, vocab) reads nothing and gives NaN. ids, logp
+ * and entropy may be NULL; top_ids / top_logp are [rows x k]; ids and top_ids are int64, the other
+ * outputs fp32. scale > 0 (1 / temperature). k <= vocab. prec 's', 'b' or 'h'. */
+int docc_b200_token_logprobs(int prec, int64_t rows, int64_t vocab, const void* X, int64_t ldx, float scale,
+                             const int64_t* ids, void* logp, void* entropy, int64_t k, int64_t* top_ids, void* top_logp, int flags);
 
 /* ---- element-wise -------------------------------------------------------------------
  * Y = act(scale * X + bias[col]) + residual over a [rows x cols] C-order tensor: the
