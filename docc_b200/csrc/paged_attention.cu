@@ -3,6 +3,19 @@
 //   s_j = scale q.k_j (capped: c tanh(s_j / c)),  p = softmax(s),  o = sum p_j v_j,  lse = log sum exp(s_j)
 //
 // docc has no such node; beside the attention entry (contiguous K and V, every query at once) this is its form for serving.
+//
+// Bound by the bytes of the cache: every key and value is used by the group = Hq / Hkv query heads that share it and by nothing
+// else, so it is read once, and the work is what keeps that stream full.
+//   * The visible tokens of a (sequence, key-value head, tile of query heads) are a row of chunks. All rows' chunks form one line,
+//     cut into as many equal runs as there are blocks: one long sequence, many short ones and any mixture load every SM alike. The
+//     lengths are read on the device, so a captured graph follows them.
+//   * A run that holds a whole row writes its output; rows that several runs share leave partial results (maximum, sum,
+//     unnormalised output) in the scratch, which a second small kernel joins in the order of the runs: no atomics, and the same
+//     result on every call.
+//   * Inside a block every warp has its own keys of each chunk, its own ring of asynchronous copies and its own running maximum and
+//     sum: nothing synchronises but the merge of the four warps at the end of a row.
+#include <type_traits>
+
 #include "common.cuh"
 #include "device_math.cuh"
 #include "ptx.cuh"
@@ -10,94 +23,877 @@
 namespace docc_b200 {
 namespace {
 
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int64_t kMostTokens = (int64_t(1) << 31) - 4096;  // token numbers of a chunk past the end still fit in 32 bits
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
 struct PagedArgs {
-    int B, Hq, Hkv, D, group;  // group = Hq / Hkv
+    int B, Hq, Hkv, D, group, tiles, tile_rows;  // group = Hq / Hkv query heads share a key-value head, in `tiles` tiles of tile_rows
+    int chunk;                                   // keys per chunk
     float scale, softcap;
     int64_t window;
     int64_t qs[2], os[2], ks[3], vs[3];  // element strides: (sequence, head), (page, head, place)
-    int64_t num_pages, page_size, max_pages, table_stride;
+    int64_t num_pages, max_pages, table_stride;
+    uint32_t page_size;
     const int32_t* page_table;
     const int32_t* lengths;
     float* lse;
     DeviceStatus* status;
+    // scratch: two partial results per block (the row it finished for an earlier block, the row it began), and per block the
+    // row it began and did not finish
+    float* part_o;    // [2 * blocks][tile_rows][D]
+    float2* part_ml;  // [2 * blocks][tile_rows]: maximum (of s log2 e), sum
+    int4* begun;      // [blocks]: {row or -1, last block of the row, 0, 0}
 };
 
 // Visible tokens [lo, n) of sequence b.
-__device__ __forceinline__ void visible(const PagedArgs& a, int b, int64_t& lo, int64_t& n) {
+__device__ __forceinline__ void visible(const PagedArgs& a, int b, int& lo, int& n) {
     n = a.lengths[b];
-    const int64_t most = a.max_pages * a.page_size;
+    int64_t most = a.max_pages * int64_t(a.page_size);
+    if (most > kMostTokens) most = kMostTokens;
     if (n < 0 || n > most) {
         report_bad_index(a.status, kIndexLength);
-        n = n < 0 ? 0 : most;
+        n = n < 0 ? 0 : int(most);
     }
-    lo = a.window > 0 && n > a.window ? n - a.window : 0;
+    lo = a.window > 0 && n > a.window ? n - int(a.window) : 0;
+}
+// An empty sequence has one chunk without visible keys, so that its output is written like any other.
+__device__ __forceinline__ int chunks_of(const PagedArgs& a, int lo, int n) { return n > lo ? (n - lo + a.chunk - 1) / a.chunk : 1; }
+
+// A place on the line of chunks: sequence-major, then key-value head, then tile of query heads, then chunk.
+struct Cursor {
+    int b, kvh, tile, chunk, chunks, lo, n;
+    __device__ __forceinline__ void enter(const PagedArgs& a) {
+        visible(a, b, lo, n);
+        chunks = chunks_of(a, lo, n);
+    }
+    __device__ __forceinline__ void next(const PagedArgs& a) {
+        if (++chunk < chunks) return;
+        chunk = 0;
+        if (++tile < a.tiles) return;
+        tile = 0;
+        if (++kvh < a.Hkv) return;
+        kvh = 0;
+        if (++b < a.B) enter(a);
+    }
+};
+
+struct Run {
+    int64_t begin, end, total;
+    int blocks;  // runs in all: never more than there are chunks, so that none is empty
+    Cursor at;
+};
+
+// The calling warp's run and its first chunk. Every warp works it out for itself, 32 sequences at a time.
+__device__ __forceinline__ bool find_run(const PagedArgs& a, Run& r) {
+    const int lane = threadIdx.x & 31;
+    const int64_t rows = int64_t(a.Hkv) * a.tiles;
+    int64_t sum = 0;
+    for (int b = lane; b < a.B; b += 32) {
+        int lo, n;
+        visible(a, b, lo, n);
+        sum += chunks_of(a, lo, n);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    r.total = sum * rows;
+    r.blocks = r.total < int64_t(gridDim.x) ? int(r.total) : int(gridDim.x);
+    if (int(blockIdx.x) >= r.blocks) return false;
+    r.begin = int64_t(blockIdx.x) * r.total / r.blocks;
+    r.end = (int64_t(blockIdx.x) + 1) * r.total / r.blocks;
+    int64_t before = 0;  // chunks of the sequences before this group of 32, times rows
+    for (int base = 0; base < a.B; base += 32) {
+        const int b = base + lane;
+        int lo = 0, n = 0;
+        int64_t mine = 0;
+        if (b < a.B) {
+            visible(a, b, lo, n);
+            mine = chunks_of(a, lo, n) * rows;
+        }
+        int64_t upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, before + upto > r.begin);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            const int64_t offset = r.begin - before - __shfl_sync(0xffffffffu, upto - mine, src);
+            r.at.b = base + src;
+            r.at.enter(a);
+            const int64_t row = offset / r.at.chunks;
+            r.at.chunk = int(offset % r.at.chunks);
+            r.at.kvh = int(row / a.tiles);
+            r.at.tile = int(row % a.tiles);
+            return true;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return false;  // not reached: begin < total
+}
+__device__ __forceinline__ int row_of(const PagedArgs& a, const Cursor& c) { return (c.b * a.Hkv + c.kvh) * a.tiles + c.tile; }
+
+// The page entry of the calling lane's key (-1: not visible).
+__device__ __forceinline__ int page_entry(const PagedArgs& a, const Cursor& c, int key) {
+    if (key >= c.n) return -1;
+    const int e = a.page_table[c.b * a.table_stride + uint32_t(key) / a.page_size];
+    if (e < 0 || e >= a.num_pages) {
+        report_bad_index(a.status, kIndexPage);
+        return -1;
+    }
+    return e;
 }
 
-// Any type, strides and size: a warp per (sequence, query head), the keys in order with the running maximum and sum.
-template <typename T, int DPL>
-__global__ void __launch_bounds__(128) paged_rows_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
-                                                         T* __restrict__ O, PagedArgs a) {
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool keep) {
+    const int bytes = keep ? 16 : 0;  // 0: the 16 bytes are filled with zeros and nothing is read
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Capped and scaled score, in units of log 2: exp(s) = 2^score.
+__device__ __forceinline__ float score_log2(const PagedArgs& a, float dot) {
+    const float s = dot * a.scale;
+    return (a.softcap > 0.f ? a.softcap * tanhf(s / a.softcap) : s) * kLog2e;
+}
+
+// ---- 16-bit inputs: tensor cores ---------------------------------------------------------------------------------------------
+// A warp step is 16 keys. S = Q K^T and O += P V run as m16n8k16 products with the (up to 16) query heads of the tile as rows: one
+// row tile is all the rows there are, and at 2 group flops per byte of cache the warp-level instruction has the rate several times
+// over, while the 128-row accumulators of tcgen05 would be 8/128 full and pay the trip through tensor memory on every step.
+// Q stays in registers, K comes as B fragments by ldmatrix, P goes from accumulator to A operand without leaving the registers.
+// P enters the product as two 16-bit parts (p = hi + lo): a single bf16 would add an error as large as the output's own rounding.
+template <typename T> __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __half>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float x, float y) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(x, y);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+// hi = the pair rounded to 16 bits, lo = what the rounding left, rounded
+template <typename T> __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+    hi = pack2<T>(x, y);
+    if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+        lo = pack2<T>(x - f.x, y - f.y);
+    } else {
+        lo = pack2<T>(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
+    }
+}
+
+template <int DP> struct TcShape {
+    static constexpr int kRow = DP * 2;                      // bytes of a key or value in shared memory
+    static constexpr int kStage = 2 * 16 * kRow;             // 16 keys and 16 values of one warp
+    static constexpr int kStages = DP <= 64 ? 5 : DP <= 96 ? 4 : 3;
+    static constexpr int kMerge = 16 * DP * 4;               // a warp's output, two of which are staged
+    static constexpr int kBytes = kWarps * kStages * kStage + 2 * kMerge;
+    // 16-byte pieces of a row are permuted so that the eight rows an ldmatrix reads at one column lie in different banks
+    static __device__ __forceinline__ uint32_t offset(int row, int piece) {
+        const int turn = DP == 96 ? (row >> 1) & 3 : row & 7;
+        return uint32_t(row * kRow + ((piece ^ turn) << 4));
+    }
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) paged_tc_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
+                                                            T* __restrict__ O, PagedArgs a) {
+    using Shape = TcShape<DP>;
+    constexpr int S = Shape::kStages, PIECES = DP / 8, NT = DP / 8;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ float2 ml_s[kWarps][16];
+    __shared__ uint32_t mask_s[kWarps][S];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    unsigned char* ring = smem + warp * (S * Shape::kStage);
+    const uint32_t ring_u = ptx::smem_u32(ring);
+    float* merge = reinterpret_cast<float*>(smem + kWarps * S * Shape::kStage);
+    const int pieces = a.D / 8;
+    if (pieces < PIECES) {  // the padding of the head is never written again
+        for (int i = lane; i < S * Shape::kStage / 16; i += 32) reinterpret_cast<uint4*>(ring)[i] = make_uint4(0, 0, 0, 0);
+        __syncwarp();
+    }
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
-    const int lane = threadIdx.x & 31;
-    const int64_t row = (int64_t(blockIdx.x) * 128 + threadIdx.x) >> 5;
-    if (row >= int64_t(a.B) * a.Hq) return;
-    const int b = int(row / a.Hq), h = int(row % a.Hq), kvh = h / a.group;
-    int64_t lo, n;
-    visible(a, b, lo, n);
-    const T* q = Q + b * a.qs[0] + h * a.qs[1];
-    float qr[DPL], acc[DPL];
-#pragma unroll
-    for (int e = 0; e < DPL; e++) {
-        const int d = lane + 32 * e;
-        qr[e] = d < a.D ? to_float(q[d]) : 0.f;
-        acc[e] = 0.f;
+
+    Run run;
+    if (!find_run(a, run)) {
+        if (threadIdx.x == 0) a.begun[blockIdx.x] = make_int4(-1, 0, 0, 0);
+        return;
     }
-    float m = -INFINITY, l = 0.f;
-    for (int64_t j = lo; j < n; j++) {
-        const int64_t page = a.page_table[b * a.table_stride + j / a.page_size], place = j % a.page_size;
-        if (page < 0 || page >= a.num_pages) {
-            report_bad_index(a.status, kIndexPage);
-            continue;
-        }
-        const T* kr = K + page * a.ks[0] + kvh * a.ks[1] + place * a.ks[2];
-        const T* vr = V + page * a.vs[0] + kvh * a.vs[1] + place * a.vs[2];
-        float s = 0.f;
+    const int units = int(run.end - run.begin);
+    Cursor load = run.at, at = run.at;
+
+    const int key_lane = warp * 16 + (lane & 15);
+    int key = load.lo + load.chunk * a.chunk + key_lane;
+    int entry = page_entry(a, load, key);
+    auto issue = [&](int stage) {  // copies of the load cursor's unit; `entry` and `key` are its own
+        const bool ok = entry >= 0;
+        const uint32_t mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+        if (lane == 0) mask_s[warp][stage] = mask;
+        if (mask) {
+            const uint32_t place = uint32_t(key) % a.page_size;
+            const int64_t ko = ok ? entry * a.ks[0] + load.kvh * a.ks[1] + place * a.ks[2] : 0;
+            const int64_t vo = ok ? entry * a.vs[0] + load.kvh * a.vs[1] + place * a.vs[2] : 0;
+            const uint32_t dst = ring_u + stage * Shape::kStage;
 #pragma unroll
-        for (int e = 0; e < DPL; e++) {
-            const int d = lane + 32 * e;
-            if (d < a.D) s = fmaf(qr[e], to_float(kr[d]), s);
+            for (int i = 0; i < 16 * PIECES / 32; i++) {
+                const int row = (i * 32 + lane) / PIECES, piece = (i * 32 + lane) % PIECES;
+                const int64_t kr = __shfl_sync(0xffffffffu, ko, row), vr = __shfl_sync(0xffffffffu, vo, row);
+                const bool keep = (mask >> row) & 1;
+                if (piece < pieces) {
+                    const uint32_t to = dst + Shape::offset(row, piece);
+                    cp_async_16(to, K + kr + piece * 8, keep);
+                    cp_async_16(to + 16 * Shape::kRow, V + vr + piece * 8, keep);
+                }
+            }
         }
-        s = warp_sum_f(s) * a.scale;
-        if (a.softcap > 0.f) s = a.softcap * tanhf(s / a.softcap);
-        const float m_new = fmaxf(m, s);
-        const float ref = m_new == -INFINITY ? 0.f : m_new;  // scores of -inf only: exp(-inf - 0) = 0, not a NaN
-        const float corr = expf(m - ref), p = expf(s - ref);
-        l = l * corr + p;
+        cp_async_commit();
+    };
+    auto advance = [&]() {  // the entry is fetched one step before its copies are issued
+        load.next(a);
+        if (load.b < a.B) {
+            key = load.lo + load.chunk * a.chunk + key_lane;
+            entry = page_entry(a, load, key);
+        }
+    };
+    int loaded = 0;
 #pragma unroll
-        for (int e = 0; e < DPL; e++) {
-            const int d = lane + 32 * e;
-            if (d < a.D) acc[e] = fmaf(p, to_float(vr[d]), acc[e] * corr);
+    for (int s = 0; s < S - 1; s++) {
+        if (loaded < units) {
+            issue(s);
+            if (++loaded < units) advance();
+        } else {
+            cp_async_commit();
         }
-        m = m_new;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    T* o = O + b * a.os[0] + h * a.os[1];
+
+    uint32_t qf[DP / 16][4];
+    float acc[NT][4], m[2], l[2];
+    int first_chunk = 0;
+    for (int u = 0; u < units; u++) {
+        if (u == 0 || at.chunk == 0) {  // a row begins
+            first_chunk = at.chunk;
+            const int r0 = at.tile * 16 + (lane >> 2);
+            const T* q0 = Q + at.b * a.qs[0] + (int64_t(at.kvh) * a.group + r0) * a.qs[1];
+            const T* q1 = q0 + 8 * a.qs[1];
 #pragma unroll
-    for (int e = 0; e < DPL; e++) {
-        const int d = lane + 32 * e;
-        if (d < a.D) o[d] = from_float<T>(acc[e] * inv);
+            for (int kk = 0; kk < DP / 16; kk++) {
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    const int d = kk * 16 + half * 8 + (lane & 3) * 2;
+                    const bool in = d < a.D;
+                    qf[kk][half * 2] = in && r0 < a.group ? *reinterpret_cast<const uint32_t*>(q0 + d) : 0u;
+                    qf[kk][half * 2 + 1] = in && r0 + 8 < a.group ? *reinterpret_cast<const uint32_t*>(q1 + d) : 0u;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NT; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[i][e] = 0.f;
+            m[0] = m[1] = -INFINITY;
+            l[0] = l[1] = 0.f;
+        }
+        cp_async_wait<S - 2>();
+        __syncwarp();  // every lane's copies of this step have landed, and every lane is done with the stage filled next
+        if (loaded < units) {
+            issue((u + S - 1) % S);
+            if (++loaded < units) advance();
+        } else {
+            cp_async_commit();
+        }
+        const int stage = u % S;
+        const uint32_t mask = mask_s[warp][stage];
+        if (mask) {
+            const uint32_t kb = ring_u + stage * Shape::kStage, vb = kb + 16 * Shape::kRow;
+            float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; kk++) {
+                uint32_t b[4];  // keys 0-7 and 8-15, dims 0-7 and 8-15 of this step
+                ldmatrix_x4(b, kb + Shape::offset((lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)));
+                mma16816<T>(s[0], qf[kk], b[0], b[1]);
+                mma16816<T>(s[1], qf[kk], b[2], b[3]);
+            }
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[t][e] = score_log2(a, s[t][e]);
+            if (mask != 0xffffu) {
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (!((mask >> (t * 8 + (lane & 3) * 2 + (e & 1))) & 1)) s[t][e] = -INFINITY;
+            }
+            float corr[2], ref[2];
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                float x = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+                const float mn = fmaxf(m[r], x);
+                ref[r] = mn == -INFINITY ? 0.f : mn;  // only scores of -inf so far: 2^(-inf - 0) = 0, not a NaN
+                corr[r] = ex2(m[r] - ref[r]);
+                m[r] = mn;
+            }
+            if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
+#pragma unroll
+                for (int i = 0; i < NT; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[i][e] *= corr[e >> 1];
+                l[0] *= corr[0];
+                l[1] *= corr[1];
+            }
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    s[t][e] = ex2(s[t][e] - ref[e >> 1]);
+                    l[e >> 1] += s[t][e];
+                }
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                split2<T>(s[t][0], s[t][1], hi[2 * t], lo[2 * t]);
+                split2<T>(s[t][2], s[t][3], hi[2 * t + 1], lo[2 * t + 1]);
+            }
+#pragma unroll
+            for (int i = 0; i < NT / 2; i++) {
+                uint32_t b[4];  // keys 0-7 and 8-15 of dims 16i..16i+7, then of the next eight
+                ldmatrix_x4_trans(b, vb + Shape::offset(lane & 15, i * 2 + (lane >> 4)));
+                mma16816<T>(acc[2 * i], hi, b[0], b[1]);
+                mma16816<T>(acc[2 * i + 1], hi, b[2], b[3]);
+                mma16816<T>(acc[2 * i], lo, b[0], b[1]);
+                mma16816<T>(acc[2 * i + 1], lo, b[2], b[3]);
+            }
+        }
+        if (at.chunk + 1 == at.chunks || u + 1 == units) {  // the row, or this block's part of it, is complete
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+                l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+            }
+            if ((lane & 3) == 0) {
+                ml_s[warp][lane >> 2] = make_float2(m[0], l[0]);
+                ml_s[warp][(lane >> 2) + 8] = make_float2(m[1], l[1]);
+            }
+            __syncthreads();
+            float total[2], top[2];
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                const int row = (lane >> 2) + 8 * r;
+                float mm = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kWarps; w++) mm = fmaxf(mm, ml_s[w][row].x);
+                const float rf = mm == -INFINITY ? 0.f : mm;
+                total[r] = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWarps; w++) total[r] += ml_s[w][row].y * ex2(ml_s[w][row].x - rf);
+                top[r] = mm;
+                const float f = ex2(m[r] - rf);
+#pragma unroll
+                for (int i = 0; i < NT; i++) {
+                    acc[i][2 * r] *= f;
+                    acc[i][2 * r + 1] *= f;
+                }
+            }
+            float* slot = merge + (warp & 1) * (16 * DP) + lane;
+            if (warp >= 2) {
+#pragma unroll
+                for (int i = 0; i < NT * 4; i++) slot[i * 32] = acc[i >> 2][i & 3];
+            }
+            __syncthreads();
+            if (warp < 2) {
+#pragma unroll
+                for (int i = 0; i < NT * 4; i++) acc[i >> 2][i & 3] += slot[i * 32];
+                if (warp == 1) {
+#pragma unroll
+                    for (int i = 0; i < NT * 4; i++) slot[i * 32] = acc[i >> 2][i & 3];
+                }
+            }
+            __syncthreads();
+            if (warp == 0) {
+                const bool whole = first_chunk == 0 && at.chunk + 1 == at.chunks;
+                const int part = 2 * blockIdx.x + (first_chunk == 0 ? 1 : 0);
+                const float* other = merge + 16 * DP + lane;
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    const int row = (lane >> 2) + 8 * r, in_group = at.tile * 16 + row;
+                    if (in_group >= a.group) continue;
+                    const int64_t head = int64_t(at.kvh) * a.group + in_group;
+                    if (whole) {
+                        const float inv = total[r] == 0.f ? 0.f : 1.f / total[r];
+                        T* o = O + at.b * a.os[0] + head * a.os[1];
+#pragma unroll
+                        for (int i = 0; i < NT; i++) {
+                            const int d = i * 8 + (lane & 3) * 2;
+                            if (d < a.D)
+                                *reinterpret_cast<uint32_t*>(o + d) = pack2<T>((acc[i][2 * r] + other[(i * 4 + 2 * r) * 32]) * inv,
+                                                                              (acc[i][2 * r + 1] + other[(i * 4 + 2 * r + 1) * 32]) * inv);
+                        }
+                        if (a.lse && (lane & 3) == 0)
+                            a.lse[at.b * int64_t(a.Hq) + head] = total[r] == 0.f ? -INFINITY : top[r] * kLn2 + logf(total[r]);
+                    } else {
+                        float* o = a.part_o + (int64_t(part) * a.tile_rows + row) * a.D;
+#pragma unroll
+                        for (int i = 0; i < NT; i++) {
+                            const int d = i * 8 + (lane & 3) * 2;
+                            if (d < a.D)
+                                *reinterpret_cast<float2*>(o + d) = make_float2(acc[i][2 * r] + other[(i * 4 + 2 * r) * 32],
+                                                                                acc[i][2 * r + 1] + other[(i * 4 + 2 * r + 1) * 32]);
+                        }
+                        if ((lane & 3) == 0) a.part_ml[int64_t(part) * a.tile_rows + row] = make_float2(top[r], total[r]);
+                    }
+                }
+                if (u + 1 == units && lane == 0) {
+                    const bool begun = first_chunk == 0 && !whole;
+                    const int64_t row_end = run.end + (at.chunks - 1 - at.chunk);
+                    a.begun[blockIdx.x] = make_int4(begun ? row_of(a, at) : -1, int((row_end * run.blocks - 1) / run.total), 0, 0);
+                }
+            }
+            __syncthreads();
+        }
+        at.next(a);
     }
-    if (a.lse && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : m + logf(l);
+}
+
+// ---- fp32, and whatever is not aligned for 16-byte copies: FMA units -------------------------------------------------------------
+// A warp step is KS keys, 32 / KS lanes to a key for the scores and DP / 32 columns to a lane for the output; keys and values are
+// staged as fp32. Up to GT query heads share the step.
+template <int DP, int GT> struct SimtShape {
+    static constexpr int kKeys = 1024 / DP;                      // 16, 8, 4
+    static constexpr int kLanes = 32 / kKeys;                    // lanes per key
+    static constexpr int kPieces = DP / 4;                       // 16-byte pieces of a row
+    static constexpr int kStage = 2 * kKeys * DP * 4;            // 8 KB
+    static constexpr int kStages = 3;
+    static constexpr int kMerge = GT * DP * 4;
+    static constexpr int kBytes = kWarps * kStages * kStage + 2 * kMerge + GT * DP * 4;
+    static __device__ __forceinline__ int offset(int row, int piece) {  // in floats; eight lanes of a step read eight banks
+        return row * DP + ((piece ^ ((row * kLanes) & 7)) << 2);
+    }
+};
+
+template <typename T, int DP, int GT, bool ASYNC>
+__global__ void __launch_bounds__(kThreads) paged_simt_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
+                                                              T* __restrict__ O, PagedArgs a) {
+    using Shape = SimtShape<DP, GT>;
+    constexpr int S = Shape::kStages, KS = Shape::kKeys, LPK = Shape::kLanes, PIECES = Shape::kPieces, C = DP / 32;
+    static_assert(!ASYNC || sizeof(T) == 4, "asynchronous copies keep the type");
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ float2 ml_s[kWarps][GT];
+    __shared__ uint32_t mask_s[kWarps][S];
+    __shared__ __align__(16) float p_s[kWarps][GT][KS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float* ring = reinterpret_cast<float*>(smem + warp * (S * Shape::kStage));
+    float* merge = reinterpret_cast<float*>(smem + kWarps * S * Shape::kStage);
+    float* q_s = merge + 2 * GT * DP;
+    if (a.D < DP) {
+        for (int i = lane; i < S * Shape::kStage / 4; i += 32) ring[i] = 0.f;
+        __syncwarp();
+    }
+    ptx::griddep_wait();
+    ptx::griddep_launch_dependents();
+
+    Run run;
+    if (!find_run(a, run)) {
+        if (threadIdx.x == 0) a.begun[blockIdx.x] = make_int4(-1, 0, 0, 0);
+        return;
+    }
+    const int units = int(run.end - run.begin);
+    Cursor load = run.at, at = run.at;
+    const int key_lane = warp * KS + (lane % KS);
+    int key = load.lo + load.chunk * a.chunk + key_lane;
+    int entry = page_entry(a, load, key);
+    auto issue = [&](int stage) {
+        const bool ok = entry >= 0;
+        const uint32_t mask = __ballot_sync(0xffffffffu, ok) & ((1u << KS) - 1u);
+        if (lane == 0) mask_s[warp][stage] = mask;
+        if (mask) {
+            const uint32_t place = uint32_t(key) % a.page_size;
+            const int64_t ko = ok ? entry * a.ks[0] + load.kvh * a.ks[1] + place * a.ks[2] : 0;
+            const int64_t vo = ok ? entry * a.vs[0] + load.kvh * a.vs[1] + place * a.vs[2] : 0;
+            float* to = ring + stage * (Shape::kStage / 4);
+            if constexpr (ASYNC) {
+                const int pieces = a.D / 4;
+#pragma unroll
+                for (int i = 0; i < KS * PIECES / 32; i++) {
+                    const int row = (i * 32 + lane) / PIECES, piece = (i * 32 + lane) % PIECES;
+                    const int64_t kr = __shfl_sync(0xffffffffu, ko, row), vr = __shfl_sync(0xffffffffu, vo, row);
+                    const bool keep = (mask >> row) & 1;
+                    if (piece < pieces) {
+                        const uint32_t dst = ptx::smem_u32(to + Shape::offset(row, piece));
+                        cp_async_16(dst, K + kr + piece * 4, keep);
+                        cp_async_16(dst + KS * DP * 4, V + vr + piece * 4, keep);
+                    }
+                }
+            } else {
+                for (int row = 0; row < KS; row++) {
+                    const int64_t kr = __shfl_sync(0xffffffffu, ko, row), vr = __shfl_sync(0xffffffffu, vo, row);
+                    const bool keep = (mask >> row) & 1;
+                    for (int d = lane; d < a.D; d += 32) {
+                        float* dst = to + Shape::offset(row, d >> 2) + (d & 3);
+                        dst[0] = keep ? to_float(K[kr + d]) : 0.f;
+                        dst[KS * DP] = keep ? to_float(V[vr + d]) : 0.f;
+                    }
+                }
+            }
+        }
+        if constexpr (ASYNC) cp_async_commit();
+    };
+    auto advance = [&]() {
+        load.next(a);
+        if (load.b < a.B) {
+            key = load.lo + load.chunk * a.chunk + key_lane;
+            entry = page_entry(a, load, key);
+        }
+    };
+    int loaded = 0;
+#pragma unroll
+    for (int s = 0; s < S - 1; s++) {
+        if (loaded < units) {
+            issue(s);
+            if (++loaded < units) advance();
+        } else if constexpr (ASYNC) {
+            cp_async_commit();
+        }
+    }
+
+    float acc[GT][C], m[GT], l[GT];
+    int first_chunk = 0;
+    for (int u = 0; u < units; u++) {
+        if (u == 0 || at.chunk == 0) {
+            first_chunk = at.chunk;
+            // the merge that ended the row before was followed by a barrier: nobody reads q_s any more
+            for (int i = threadIdx.x; i < GT * DP; i += kThreads) {
+                const int g = i / DP, d = i % DP, in_group = at.tile * GT + g;
+                q_s[i] = d < a.D && in_group < a.group
+                             ? to_float(Q[at.b * a.qs[0] + (int64_t(at.kvh) * a.group + in_group) * a.qs[1] + d])
+                             : 0.f;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int g = 0; g < GT; g++) {
+#pragma unroll
+                for (int c = 0; c < C; c++) acc[g][c] = 0.f;
+                m[g] = -INFINITY;
+                l[g] = 0.f;
+            }
+        }
+        if constexpr (ASYNC) cp_async_wait<S - 2>();
+        __syncwarp();
+        if (loaded < units) {
+            issue((u + S - 1) % S);
+            if (++loaded < units) advance();
+        } else if constexpr (ASYNC) {
+            cp_async_commit();
+        }
+        const int stage = u % S;
+        const uint32_t mask = mask_s[warp][stage];
+        if (mask) {
+            const float* kb = ring + stage * (Shape::kStage / 4);
+            const float* vb = kb + KS * DP;
+            const int my_key = lane / LPK, sub = lane % LPK;
+            float s[GT];
+#pragma unroll
+            for (int g = 0; g < GT; g++) s[g] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int piece = i * LPK + sub;
+                const float4 k4 = *reinterpret_cast<const float4*>(kb + Shape::offset(my_key, piece));
+#pragma unroll
+                for (int g = 0; g < GT; g++) {
+                    const float4 q4 = *reinterpret_cast<const float4*>(q_s + g * DP + piece * 4);
+                    s[g] = fmaf(k4.x, q4.x, fmaf(k4.y, q4.y, fmaf(k4.z, q4.z, fmaf(k4.w, q4.w, s[g]))));
+                }
+            }
+            const bool seen = (mask >> my_key) & 1;
+            __syncwarp();  // p_s of the step before has been read
+#pragma unroll
+            for (int g = 0; g < GT; g++) {
+                float x = s[g];
+#pragma unroll
+                for (int o = 1; o < LPK; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+                x = seen ? score_log2(a, x) : -INFINITY;
+                float t = x;
+#pragma unroll
+                for (int o = LPK; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+                const float mn = fmaxf(m[g], t), ref = mn == -INFINITY ? 0.f : mn;
+                const float corr = ex2(m[g] - ref), p = ex2(x - ref);
+                m[g] = mn;
+                l[g] = l[g] * corr + (sub == 0 ? p : 0.f);
+#pragma unroll
+                for (int c = 0; c < C; c++) acc[g][c] *= corr;
+                if (sub == 0) p_s[warp][g][my_key] = p;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int j4 = 0; j4 < KS / 4; j4++) {
+                float v[4][C];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int row = j4 * 4 + j;
+                    if constexpr (C == 2) {
+                        const float2 f = *reinterpret_cast<const float2*>(vb + Shape::offset(row, lane >> 1) + (lane & 1) * 2);
+                        v[j][0] = f.x; v[j][1] = f.y;
+                    } else {
+#pragma unroll
+                        for (int h = 0; h < C / 4; h++) {
+                            const float4 f = *reinterpret_cast<const float4*>(vb + Shape::offset(row, lane + 32 * h));
+                            v[j][4 * h] = f.x; v[j][4 * h + 1] = f.y; v[j][4 * h + 2] = f.z; v[j][4 * h + 3] = f.w;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int g = 0; g < GT; g++) {
+                    const float4 p4 = *reinterpret_cast<const float4*>(&p_s[warp][g][j4 * 4]);
+#pragma unroll
+                    for (int c = 0; c < C; c++)
+                        acc[g][c] = fmaf(p4.x, v[0][c], fmaf(p4.y, v[1][c], fmaf(p4.z, v[2][c], fmaf(p4.w, v[3][c], acc[g][c]))));
+                }
+            }
+        }
+        if (at.chunk + 1 == at.chunks || u + 1 == units) {
+#pragma unroll
+            for (int g = 0; g < GT; g++) {
+                l[g] = warp_sum_f(l[g]);
+                if (lane == 0) ml_s[warp][g] = make_float2(m[g], l[g]);
+            }
+            __syncthreads();
+            float total[GT], top[GT];
+#pragma unroll
+            for (int g = 0; g < GT; g++) {
+                float mm = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kWarps; w++) mm = fmaxf(mm, ml_s[w][g].x);
+                const float rf = mm == -INFINITY ? 0.f : mm;
+                total[g] = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWarps; w++) total[g] += ml_s[w][g].y * ex2(ml_s[w][g].x - rf);
+                top[g] = mm;
+                const float f = ex2(m[g] - rf);
+#pragma unroll
+                for (int c = 0; c < C; c++) acc[g][c] *= f;
+            }
+            float* slot = merge + (warp & 1) * (GT * DP) + lane;
+            if (warp >= 2) {
+#pragma unroll
+                for (int i = 0; i < GT * C; i++) slot[i * 32] = acc[i / C][i % C];
+            }
+            __syncthreads();
+            if (warp < 2) {
+#pragma unroll
+                for (int i = 0; i < GT * C; i++) acc[i / C][i % C] += slot[i * 32];
+                if (warp == 1) {
+#pragma unroll
+                    for (int i = 0; i < GT * C; i++) slot[i * 32] = acc[i / C][i % C];
+                }
+            }
+            __syncthreads();
+            if (warp == 0) {
+                const bool whole = first_chunk == 0 && at.chunk + 1 == at.chunks;
+                const int part = 2 * blockIdx.x + (first_chunk == 0 ? 1 : 0);
+                const float* other = merge + GT * DP + lane;
+#pragma unroll
+                for (int g = 0; g < GT; g++) {
+                    const int in_group = at.tile * GT + g;
+                    if (in_group >= a.group) continue;
+                    const int64_t head = int64_t(at.kvh) * a.group + in_group;
+                    const float inv = !whole ? 1.f : total[g] == 0.f ? 0.f : 1.f / total[g];
+#pragma unroll
+                    for (int c = 0; c < C; c++) {
+                        const int d = C == 2 ? lane * 2 + c : (c >> 2) * 128 + lane * 4 + (c & 3);
+                        if (d >= a.D) continue;
+                        const float o = (acc[g][c] + other[(g * C + c) * 32]) * inv;
+                        if (whole) O[at.b * a.os[0] + head * a.os[1] + d] = from_float<T>(o);
+                        else a.part_o[(int64_t(part) * a.tile_rows + g) * a.D + d] = o;
+                    }
+                    if (lane == 0) {
+                        if (!whole) a.part_ml[int64_t(part) * a.tile_rows + g] = make_float2(top[g], total[g]);
+                        else if (a.lse)
+                            a.lse[at.b * int64_t(a.Hq) + head] = total[g] == 0.f ? -INFINITY : top[g] * kLn2 + logf(total[g]);
+                    }
+                }
+                if (u + 1 == units && lane == 0) {
+                    const bool begun = first_chunk == 0 && !whole;
+                    const int64_t row_end = run.end + (at.chunks - 1 - at.chunk);
+                    a.begun[blockIdx.x] = make_int4(begun ? row_of(a, at) : -1, int((row_end * run.blocks - 1) / run.total), 0, 0);
+                }
+            }
+            __syncthreads();
+        }
+        at.next(a);
+    }
+}
+
+// ---- join ----------------------------------------------------------------------------------------------------------------------
+// Block (c, r): query head r of the row that block c of the first kernel began and did not finish; its parts lie in the blocks up to
+// `last`, the first as the row begun, the others as the row finished for an earlier block. Four groups of threads take every fourth
+// part.
+constexpr int kJoinGroups = 4;
+template <typename T, int DP>
+__global__ void __launch_bounds__(kJoinGroups * DP) paged_join_kernel(T* __restrict__ O, PagedArgs a) {
+    extern __shared__ float weight_s[];  // one per part
+    __shared__ float red[kJoinGroups][DP];
+    __shared__ float total_s;
+    ptx::griddep_wait();
+    ptx::griddep_launch_dependents();
+    const int4 begun = a.begun[blockIdx.x];
+    if (begun.x < 0) return;
+    const int r = blockIdx.y, tile = begun.x % a.tiles, in_group = tile * a.tile_rows + r;
+    if (in_group >= a.group) return;
+    const int kvh = begun.x / a.tiles % a.Hkv, b = begun.x / a.tiles / a.Hkv;
+    const int parts = begun.y - int(blockIdx.x) + 1;
+    auto part = [&](int i) { return int64_t(2 * (int(blockIdx.x) + i) + (i == 0 ? 1 : 0)) * a.tile_rows + r; };
+    if (threadIdx.x < 32) {
+        float top = -INFINITY, sum = 0.f;
+        for (int i = threadIdx.x; i < parts; i += 32) top = fmaxf(top, a.part_ml[part(i)].x);
+        top = warp_max_f(top);
+        const float ref = top == -INFINITY ? 0.f : top;
+        for (int i = threadIdx.x; i < parts; i += 32) {
+            const float2 ml = a.part_ml[part(i)];
+            const float w = ex2(ml.x - ref);
+            weight_s[i] = w;
+            sum += w * ml.y;
+        }
+        sum = warp_sum_f(sum);
+        if (threadIdx.x == 0) {
+            total_s = sum;
+            if (a.lse) a.lse[b * int64_t(a.Hq) + int64_t(kvh) * a.group + in_group] = sum == 0.f ? -INFINITY : top * kLn2 + logf(sum);
+        }
+    }
+    __syncthreads();
+    const int d = threadIdx.x % DP, group = threadIdx.x / DP;
+    float o = 0.f;
+    if (d < a.D) {
+#pragma unroll 8
+        for (int i = group; i < parts; i += kJoinGroups) {
+            const float w = weight_s[i];
+            if (w != 0.f) o = fmaf(w, a.part_o[part(i) * a.D + d], o);
+        }
+    }
+    red[group][d] = o;
+    __syncthreads();
+    if (group == 0 && d < a.D) {
+#pragma unroll
+        for (int g = 1; g < kJoinGroups; g++) o += red[g][d];
+        O[b * a.os[0] + (int64_t(kvh) * a.group + in_group) * a.os[1] + d] = from_float<T>(total_s == 0.f ? 0.f : o / total_s);
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------
+constexpr int kTcRows = 16, kSimtRows = 8;
+
+struct Scratch {
+    size_t ml_at, o_at, bytes;
+};
+Scratch scratch_of(int blocks, int64_t group, int64_t D) {
+    // the larger of the two kernels' tiles, so that the size does not depend on alignment
+    const size_t rows = size_t(group < kTcRows ? group : kTcRows), parts = 2 * size_t(blocks);
+    Scratch s;
+    s.ml_at = (size_t(blocks) * sizeof(int4) + 255) / 256 * 256;
+    s.o_at = s.ml_at + (parts * rows * sizeof(float2) + 255) / 256 * 256;
+    s.bytes = s.o_at + parts * rows * size_t(D) * 4;
+    return s;
+}
+int blocks_of(Ctx* ctx, int64_t D) { return ctx->sm_count * (D <= 128 ? 2 : 1); }
+
+template <typename F> int set_smem(F kernel, int bytes) {
+    DOCC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    return DOCC_B200_OK;
 }
 
 template <typename T>
-int paged_device(Ctx* ctx, const PagedArgs& a, const void* Q, const void* K, const void* V, void* O) {
-    const dim3 grid(unsigned(ceil_div(int64_t(a.B) * a.Hq, 4)));
-    auto kernel = a.D <= 64 ? paged_rows_kernel<T, 2> : a.D <= 128 ? paged_rows_kernel<T, 4> : paged_rows_kernel<T, 8>;
-    DOCC_CUDA_TRY(launch_pdl(kernel, grid, dim3(128), 0, ctx->stream, static_cast<const T*>(Q), static_cast<const T*>(K),
-                             static_cast<const T*>(V), static_cast<T*>(O), a));
-    return after_launch(ctx, "paged_rows_kernel");
+int launch_join(Ctx* ctx, const PagedArgs& a, int blocks, T* O) {
+    const dim3 grid(unsigned(blocks), unsigned(a.group < a.tile_rows ? a.group : a.tile_rows));
+    const size_t smem = size_t(blocks) * 4;
+    if (a.D <= 64) DOCC_CUDA_TRY(launch_pdl(paged_join_kernel<T, 64>, grid, dim3(kJoinGroups * 64), smem, ctx->stream, O, a));
+    else if (a.D <= 128) DOCC_CUDA_TRY(launch_pdl(paged_join_kernel<T, 128>, grid, dim3(kJoinGroups * 128), smem, ctx->stream, O, a));
+    else DOCC_CUDA_TRY(launch_pdl(paged_join_kernel<T, 256>, grid, dim3(kJoinGroups * 256), smem, ctx->stream, O, a));
+    return after_launch(ctx, "paged_join_kernel");
+}
+
+template <typename T, int DP>
+int launch_tc(Ctx* ctx, PagedArgs& a, int blocks, const T* Q, const T* K, const T* V, T* O) {
+    a.tile_rows = kTcRows;
+    a.tiles = int(ceil_div(a.group, kTcRows));
+    if (a.tiles == 1) a.tile_rows = a.group;  // the scratch holds no rows that do not exist
+    a.chunk = kWarps * 16;
+    auto kernel = paged_tc_kernel<T, DP>;
+    DOCC_TRY(set_smem(kernel, TcShape<DP>::kBytes));
+    DOCC_CUDA_TRY(launch_pdl(kernel, dim3(unsigned(blocks)), dim3(kThreads), TcShape<DP>::kBytes, ctx->stream, Q, K, V, O, a));
+    DOCC_TRY(after_launch(ctx, "paged_tc_kernel"));
+    return launch_join<T>(ctx, a, blocks, O);
+}
+
+template <typename T, int DP, int GT, bool ASYNC>
+int launch_simt(Ctx* ctx, PagedArgs& a, int blocks, const T* Q, const T* K, const T* V, T* O) {
+    a.tile_rows = GT;
+    a.tiles = int(ceil_div(a.group, GT));
+    if (a.tiles == 1) a.tile_rows = a.group;
+    a.chunk = kWarps * SimtShape<DP, GT>::kKeys;
+    auto kernel = paged_simt_kernel<T, DP, GT, ASYNC>;
+    DOCC_TRY(set_smem(kernel, SimtShape<DP, GT>::kBytes));
+    DOCC_CUDA_TRY(launch_pdl(kernel, dim3(unsigned(blocks)), dim3(kThreads), SimtShape<DP, GT>::kBytes, ctx->stream, Q, K, V, O, a));
+    DOCC_TRY(after_launch(ctx, "paged_simt_kernel"));
+    return launch_join<T>(ctx, a, blocks, O);
+}
+template <typename T, int DP, bool ASYNC>
+int launch_simt_rows(Ctx* ctx, PagedArgs& a, int blocks, const T* Q, const T* K, const T* V, T* O) {
+    if (a.group == 1) return launch_simt<T, DP, 1, ASYNC>(ctx, a, blocks, Q, K, V, O);
+    if (a.group <= 4) return launch_simt<T, DP, 4, ASYNC>(ctx, a, blocks, Q, K, V, O);
+    return launch_simt<T, DP, kSimtRows, ASYNC>(ctx, a, blocks, Q, K, V, O);
+}
+template <typename T, bool ASYNC>
+int launch_simt_any(Ctx* ctx, PagedArgs& a, int blocks, const T* Q, const T* K, const T* V, T* O) {
+    if (a.D <= 64) return launch_simt_rows<T, 64, ASYNC>(ctx, a, blocks, Q, K, V, O);
+    if (a.D <= 128) return launch_simt_rows<T, 128, ASYNC>(ctx, a, blocks, Q, K, V, O);
+    return launch_simt_rows<T, 256, ASYNC>(ctx, a, blocks, Q, K, V, O);
+}
+
+template <typename T>
+int paged_device(Ctx* ctx, PagedArgs& a, int blocks, const void* Qv, const void* Kv, const void* Vv, void* Ov) {
+    const T *Q = static_cast<const T*>(Qv), *K = static_cast<const T*>(Kv), *V = static_cast<const T*>(Vv);
+    T* O = static_cast<T*>(Ov);
+    constexpr int VEC = 16 / sizeof(T);
+    bool aligned = a.D % VEC == 0;
+    for (const void* p : {Qv, Kv, Vv, static_cast<const void*>(Ov)}) aligned = aligned && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+    for (int i = 0; i < 2; i++) aligned = aligned && a.qs[i] % VEC == 0 && a.os[i] % VEC == 0;
+    for (int i = 0; i < 3; i++) aligned = aligned && a.ks[i] % VEC == 0 && a.vs[i] % VEC == 0;
+    if constexpr (sizeof(T) == 2) {
+        if (aligned) {
+            if (a.D <= 64) return launch_tc<T, 64>(ctx, a, blocks, Q, K, V, O);
+            if (a.D <= 96) return launch_tc<T, 96>(ctx, a, blocks, Q, K, V, O);
+            if (a.D <= 128) return launch_tc<T, 128>(ctx, a, blocks, Q, K, V, O);
+            return launch_tc<T, 256>(ctx, a, blocks, Q, K, V, O);
+        }
+    } else {
+        if (aligned) return launch_simt_any<T, true>(ctx, a, blocks, Q, K, V, O);
+    }
+    return launch_simt_any<T, false>(ctx, a, blocks, Q, K, V, O);
 }
 
 }  // namespace
@@ -109,7 +905,9 @@ extern "C" int docc_b200_paged_attention_workspace(int prec, int64_t B, int64_t 
     DOCC_REQUIRE(bytes != nullptr, "paged_attention_workspace: bytes is NULL");
     DOCC_REQUIRE(prec_size(prec) != 0 && prec != DOCC_B200_PREC_D, "paged_attention_workspace: precision %d not supported (use 's', 'b' or 'h')", prec);
     DOCC_REQUIRE(B >= 0 && Hq >= 0 && Hkv >= 0 && D >= 0, "paged_attention_workspace: negative extent");
-    *bytes = 0;
+    Ctx* ctx;
+    DOCC_TRY(get_ctx(&ctx));
+    *bytes = B == 0 || Hkv == 0 || D == 0 ? 0 : scratch_of(blocks_of(ctx, D), Hq / Hkv, D).bytes;
     return DOCC_B200_OK;
 }
 
@@ -133,10 +931,19 @@ extern "C" int docc_b200_paged_attention(int prec, int64_t B, int64_t Hq, int64_
                  (long long)Hkv);
     if (D > 256) return set_error(DOCC_B200_ERR_UNSUPPORTED, "paged_attention: head_dim %lld > 256", (long long)D);
     DOCC_REQUIRE(B <= 65535 && Hq <= 65535, "paged_attention: more than 65535 sequences or heads");
+    DOCC_REQUIRE(B * Hq < (int64_t(1) << 31), "paged_attention: 2^31 or more rows");
     DOCC_REQUIRE(Q && O && lengths && (max_pages == 0 || (page_table && (num_pages == 0 || (Kcache && Vcache)))),
                  "paged_attention: NULL data pointer");
     DOCC_REQUIRE(table_stride >= max_pages, "paged_attention: table_stride below max_pages");
-    (void)workspace; (void)workspace_bytes;
+    DOCC_REQUIRE(page_size < (int64_t(1) << 31), "paged_attention: page_size of 2^31 or more");
+    const int blocks = blocks_of(ctx, D);
+    const Scratch scratch = scratch_of(blocks, Hq / Hkv, D);
+    if (workspace) {
+        DOCC_REQUIRE(workspace_bytes >= scratch.bytes && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
+                     "paged_attention: the workspace needs %zu bytes on a 16-byte boundary", scratch.bytes);
+    } else {
+        DOCC_TRY(get_workspace(ctx, 3, scratch.bytes, &workspace));
+    }
     PagedArgs a;
     a.B = int(B); a.Hq = int(Hq); a.Hkv = int(Hkv); a.D = int(D); a.group = int(Hq / Hkv);
     a.scale = scale; a.softcap = softcap; a.window = window;
@@ -147,9 +954,14 @@ extern "C" int docc_b200_paged_attention(int prec, int64_t B, int64_t Hq, int64_
         a.ks[i] = kc_strides ? kc_strides[i] : dense[i];
         a.vs[i] = vc_strides ? vc_strides[i] : dense[i];
     }
-    a.num_pages = num_pages; a.page_size = page_size; a.max_pages = max_pages; a.table_stride = table_stride;
+    a.num_pages = num_pages; a.page_size = uint32_t(page_size); a.max_pages = max_pages; a.table_stride = table_stride;
     a.page_table = page_table; a.lengths = lengths; a.lse = static_cast<float*>(lse); a.status = ctx->status_dev;
-    if (prec == DOCC_B200_PREC_S) return paged_device<float>(ctx, a, Q, Kcache, Vcache, O);
-    if (prec == DOCC_B200_PREC_H) return paged_device<__half>(ctx, a, Q, Kcache, Vcache, O);
-    return paged_device<__nv_bfloat16>(ctx, a, Q, Kcache, Vcache, O);
+    a.begun = static_cast<int4*>(workspace);
+    a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + scratch.ml_at);
+    a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + scratch.o_at);
+    if (!Kcache) Kcache = Q;  // an empty cache: nothing of it is read, but copies of no bytes want an address
+    if (!Vcache) Vcache = Q;
+    if (prec == DOCC_B200_PREC_S) return paged_device<float>(ctx, a, blocks, Q, Kcache, Vcache, O);
+    if (prec == DOCC_B200_PREC_H) return paged_device<__half>(ctx, a, blocks, Q, Kcache, Vcache, O);
+    return paged_device<__nv_bfloat16>(ctx, a, blocks, Q, Kcache, Vcache, O);
 }
