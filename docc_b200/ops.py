@@ -98,17 +98,34 @@ class DeviceArray:
             self._ptr = None
 
 
+_torch_types = {}  # type -> whether torch defines it
+
+
 def _is_torch(x) -> bool:
-    return type(x).__module__.startswith("torch")
+    kind = type(x)
+    known = _torch_types.get(kind)
+    if known is None:
+        known = _torch_types[kind] = kind.__module__.startswith("torch")
+    return known
+
+
+_type_names = {}  # dtype of either library -> its name
+
+
+def _type_name(dtype) -> str:
+    name = _type_names.get(dtype)
+    if name is None:
+        name = _type_names[dtype] = str(dtype)[6:] if str(dtype).startswith("torch.") else np.dtype(dtype).name
+    return name
+
+
+_PRECISIONS = {"float64": ord("d"), "float32": ord("s"), "float16": ord("h"), "bfloat16": ord("b")}
 
 
 def _prec(x) -> int:
-    if _is_torch(x):
-        name = str(x.dtype).replace("torch.", "")
-    else:
-        name = np.dtype(x.dtype).name  # numpy arrays and DeviceArrays
+    name = _type_name(x.dtype)
     try:
-        return {"float64": ord("d"), "float32": ord("s"), "float16": ord("h"), "bfloat16": ord("b")}[name]
+        return _PRECISIONS[name]
     except KeyError:
         raise TypeError(f"unsupported element type {name}") from None
 
@@ -342,39 +359,30 @@ def layernorm(X, gamma=None, beta=None, eps=1e-5, flags=0):
 def _side(*xs):
     """``_kind`` without its demand for contiguity, for entries that take strides: flags, after checking that all arrays live on the
     same side and, for torch tensors, on the device that the calling thread's launches go to."""
-    xs = [x for x in xs if x is not None]
-    device = [_is_torch(x) or isinstance(x, DeviceArray) for x in xs]
-    if not any(device):
-        for x in xs:
-            if not x.flags["C_CONTIGUOUS"]:
-                raise ValueError("arrays must be C-contiguous")
-        return FLAG_HOST_PTRS
-    if not all(device):
-        raise TypeError("mix of host arrays and device tensors")
+    host = device = 0
     current = None
     for x in xs:
-        if not _is_torch(x):
+        if x is None:
             continue
-        if not x.is_cuda:
-            raise TypeError("torch tensors must live on a CUDA device (pass numpy arrays for host data)")
-        if current is None:
-            import torch
+        if _is_torch(x):
+            if not x.is_cuda:
+                raise TypeError("torch tensors must live on a CUDA device (pass numpy arrays for host data)")
+            if current is None:
+                import torch
 
-            current = torch.cuda.current_device()
-        if x.get_device() != current:
-            raise ValueError(f"tensor on cuda:{x.get_device()} while the calling thread's device is cuda:{current}")
-    return 0
-
-
-def _strides(x):
-    """Element strides of all dimensions."""
-    if _is_torch(x):
-        return x.stride()
-    out, n = [], 1
-    for s in reversed(x.shape):
-        out.append(n)
-        n *= int(s)
-    return tuple(reversed(out))
+                current = torch.cuda.current_device()
+            if x.get_device() != current:
+                raise ValueError(f"tensor on cuda:{x.get_device()} while the calling thread's device is cuda:{current}")
+            device += 1
+        elif isinstance(x, DeviceArray):
+            device += 1
+        else:
+            if not x.flags["C_CONTIGUOUS"]:
+                raise ValueError("arrays must be C-contiguous")
+            host += 1
+    if host and device:
+        raise TypeError("mix of host arrays and device tensors")
+    return FLAG_HOST_PTRS if host else 0
 
 
 def _heads_strides(x, name, written=False):
@@ -413,9 +421,8 @@ def _rows_of(x, name):
 
 
 def _want(x, dtype, name, shape=None):
-    got = str(x.dtype).replace("torch.", "") if _is_torch(x) else np.dtype(x.dtype).name
-    if got != dtype:
-        raise TypeError(f"{name} must be {dtype}, not {got}")
+    if _type_name(x.dtype) != dtype:
+        raise TypeError(f"{name} must be {dtype}, not {_type_name(x.dtype)}")
     if shape is not None and tuple(x.shape) != tuple(shape):
         raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(x.shape)}")
     if _is_torch(x) and not x.is_contiguous():
