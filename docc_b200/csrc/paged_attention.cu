@@ -14,6 +14,7 @@
 //     result on every call.
 //   * Inside a block every warp has its own keys of each chunk, its own ring of asynchronous copies and its own running maximum and
 //     sum: nothing synchronises but the merge of the four warps at the end of a row.
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -821,8 +822,12 @@ Scratch scratch_of(int blocks, int64_t group, int64_t D) {
 }
 int blocks_of(Ctx* ctx, int64_t D) { return ctx->sm_count * (D <= 128 ? 2 : 1); }
 
-template <typename F> int set_smem(F kernel, int bytes) {
+// The attribute is set once per kernel and device: `done` is the caller's, one per kernel.
+template <typename F> int set_smem(Ctx* ctx, std::atomic<unsigned>& done, F kernel, int bytes) {
+    const unsigned bit = 1u << ctx->device;  // fewer than 16 devices
+    if (done.load(std::memory_order_acquire) & bit) return DOCC_B200_OK;
     DOCC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(bit, std::memory_order_release);
     return DOCC_B200_OK;
 }
 
@@ -843,7 +848,8 @@ int launch_tc(Ctx* ctx, PagedArgs& a, int blocks, const T* Q, const T* K, const 
     if (a.tiles == 1) a.tile_rows = a.group;  // the scratch holds no rows that do not exist
     a.chunk = kWarps * 16;
     auto kernel = paged_tc_kernel<T, DP>;
-    DOCC_TRY(set_smem(kernel, TcShape<DP>::kBytes));
+    static std::atomic<unsigned> done{0};
+    DOCC_TRY(set_smem(ctx, done, kernel, TcShape<DP>::kBytes));
     DOCC_CUDA_TRY(launch_pdl(kernel, dim3(unsigned(blocks)), dim3(kThreads), TcShape<DP>::kBytes, ctx->stream, Q, K, V, O, a));
     DOCC_TRY(after_launch(ctx, "paged_tc_kernel"));
     return launch_join<T>(ctx, a, blocks, O);
@@ -856,7 +862,8 @@ int launch_simt(Ctx* ctx, PagedArgs& a, int blocks, const T* Q, const T* K, cons
     if (a.tiles == 1) a.tile_rows = a.group;
     a.chunk = kWarps * SimtShape<DP, GT>::kKeys;
     auto kernel = paged_simt_kernel<T, DP, GT, ASYNC>;
-    DOCC_TRY(set_smem(kernel, SimtShape<DP, GT>::kBytes));
+    static std::atomic<unsigned> done{0};
+    DOCC_TRY(set_smem(ctx, done, kernel, SimtShape<DP, GT>::kBytes));
     DOCC_CUDA_TRY(launch_pdl(kernel, dim3(unsigned(blocks)), dim3(kThreads), SimtShape<DP, GT>::kBytes, ctx->stream, Q, K, V, O, a));
     DOCC_TRY(after_launch(ctx, "paged_simt_kernel"));
     return launch_join<T>(ctx, a, blocks, O);

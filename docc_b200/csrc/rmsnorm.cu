@@ -34,12 +34,135 @@ __device__ __forceinline__ uint8_t quantise(float y, float scale) {
     return __nv_cvt_float_to_fp8(scale == 0.f ? 0.f : __fdiv_rn(y, scale), __NV_SATFINITE, __NV_E4M3);
 }
 
+template <int N> __device__ __forceinline__ void store_codes(uint8_t* q, const float (&y)[N], float scale) {
+    Pack<uint8_t, N> c;  // N-byte aligned: cols and the row's first code are multiples of N
+#pragma unroll
+    for (int e = 0; e < N; e++) c.v[e] = quantise(y[e], scale);
+    *reinterpret_cast<Pack<uint8_t, N>*>(q) = c;
+}
+
 struct RmsArgs {
     int64_t rows, cols, ldx, ldr;
     float eps;
     const float* gamma;
     int64_t group;  // 8-bit output: columns per scale
 };
+
+// Rows whose operands are aligned for 16-byte accesses: TPR threads to a row, which stays in registers (VPT packs each).
+template <typename T, bool Q8, int TPR, int VPT>
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) rmsnorm_kernel(const T* X, const T* R, T* S, T* Y, uint8_t* Q, float* scales,
+                                                                       RmsArgs a) {
+    ptx::griddep_wait();
+    ptx::griddep_launch_dependents();
+    constexpr int VEC = 16 / sizeof(T), BLOCK = TPR < 128 ? 128 : TPR, RPB = BLOCK / TPR, WPR = TPR / 32;
+    constexpr int LANES = kRmsGroup / VEC;  // lanes that hold a group of columns: 16 or 32
+    using P = Pack<T, VEC>;
+    __shared__ float red[2][RPB][WPR];
+    const int t = threadIdx.x % TPR, rib = threadIdx.x / TPR, wir = t / 32, lane = threadIdx.x & 31;
+    const int packs = int(a.cols / VEC);
+    const int64_t row = int64_t(blockIdx.x) * RPB + rib;
+    const bool ok = row < a.rows;
+    const P* x = reinterpret_cast<const P*>(X + row * a.ldx);
+    const P* r = reinterpret_cast<const P*>(R + row * a.ldr);
+    P px[VPT], pr[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; i++)
+        if (ok && i * TPR + t < packs) px[i] = load_pack(x + i * TPR + t);
+    if (R) {
+#pragma unroll
+        for (int i = 0; i < VPT; i++)
+            if (ok && i * TPR + t < packs) pr[i] = load_pack(r + i * TPR + t);
+    }
+    float v[VPT][VEC];
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; i++) {
+        const int p = i * TPR + t;
+        const bool in = ok && p < packs;
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            v[i][e] = in ? to_float(px[i].v[e]) : 0.f;
+            if (R && in) v[i][e] += to_float(pr[i].v[e]);
+            ss = fmaf(v[i][e], v[i][e], ss);
+        }
+        if (S && in) {
+            P ps;
+#pragma unroll
+            for (int e = 0; e < VEC; e++) ps.v[e] = from_float<T>(v[i][e]);
+            store_pack(reinterpret_cast<P*>(S + row * a.cols) + p, ps);
+        }
+    }
+    ss = warp_sum_f(ss);
+    if constexpr (WPR > 1) {
+        if (lane == 0) red[0][rib][wir] = ss;
+        __syncthreads();
+        ss = 0.f;
+#pragma unroll
+        for (int w = 0; w < WPR; w++) ss += red[0][rib][w];
+    }
+    const float rstd = rsqrtf(ss / float(a.cols) + a.eps);
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; i++) {
+        const int p = i * TPR + t;
+        float g[VEC];
+        if (a.gamma && p < packs) {
+#pragma unroll
+            for (int h = 0; h < VEC / 4; h++) {
+                const float4 f = __ldg(reinterpret_cast<const float4*>(a.gamma) + p * (VEC / 4) + h);
+                g[4 * h] = f.x; g[4 * h + 1] = f.y; g[4 * h + 2] = f.z; g[4 * h + 3] = f.w;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; e++) g[e] = 1.f;
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; e++) v[i][e] = v[i][e] * rstd * g[e];
+        if constexpr (!Q8) {
+            if (ok && p < packs) {
+                P py;
+#pragma unroll
+                for (int e = 0; e < VEC; e++) py.v[e] = from_float<T>(v[i][e]);
+                store_pack(reinterpret_cast<P*>(Y + row * a.cols) + p, py);
+            }
+        } else if (p < packs) {  // 0 * inf in a column that does not exist would be a NaN
+#pragma unroll
+            for (int e = 0; e < VEC; e++) top = max_nan(top, fabsf(v[i][e]));
+        }
+        if constexpr (Q8) {
+            if (a.group < a.cols) {
+                float m = top;
+                top = 0.f;
+#pragma unroll
+                for (int o = LANES / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+                const float scale = __fdiv_rn(m, kE4m3Max);
+                if (ok && p < packs) {
+                    store_codes<VEC>(Q + row * a.cols + int64_t(p) * VEC, v[i], scale);
+                    if (lane % LANES == 0) scales[row * ((a.cols + kRmsGroup - 1) / kRmsGroup) + p / LANES] = scale;
+                }
+            }
+        }
+    }
+    if constexpr (Q8) {
+        if (a.group >= a.cols) {
+            top = warp_max_nan(top);
+            if constexpr (WPR > 1) {
+                if (lane == 0) red[1][rib][wir] = top;
+                __syncthreads();
+                top = red[1][rib][0];
+#pragma unroll
+                for (int w = 1; w < WPR; w++) top = max_nan(top, red[1][rib][w]);
+            }
+            const float scale = __fdiv_rn(top, kE4m3Max);
+#pragma unroll
+            for (int i = 0; i < VPT; i++) {
+                const int p = i * TPR + t;
+                if (ok && p < packs) store_codes<VEC>(Q + row * a.cols + int64_t(p) * VEC, v[i], scale);
+            }
+            if (ok && t == 0) scales[row] = scale;
+        }
+    }
+}
 
 // Any width and alignment: one block per row, the row staged in shared memory.
 template <typename T, bool Q8>
@@ -54,6 +177,7 @@ __global__ void __launch_bounds__(256) rmsnorm_row_kernel(const T* X, const T* R
         const T* x = X + row * a.ldx;
         const T* r = R ? R + row * a.ldr : nullptr;
         float ss = 0.f;
+#pragma unroll 8
         for (int c = t; c < cols; c += 256) {
             float v = to_float(x[c]);
             if (r) v += to_float(r[c]);
@@ -111,8 +235,31 @@ __global__ void __launch_bounds__(256) rmsnorm_row_kernel(const T* X, const T* R
     }
 }
 
+template <typename T, bool Q8, int TPR, int VPT>
+int launch_rms(Ctx* ctx, const RmsArgs& a, const void* X, const void* R, void* S, void* Y, void* Q, void* scales) {
+    constexpr int BLOCK = TPR < 128 ? 128 : TPR;
+    DOCC_CUDA_TRY(launch_pdl(rmsnorm_kernel<T, Q8, TPR, VPT>, dim3(unsigned(ceil_div(a.rows, BLOCK / TPR))), dim3(BLOCK), 0, ctx->stream,
+                             static_cast<const T*>(X), static_cast<const T*>(R), static_cast<T*>(S), static_cast<T*>(Y),
+                             static_cast<uint8_t*>(Q), static_cast<float*>(scales), a));
+    return after_launch(ctx, "rmsnorm_kernel");
+}
+
 template <typename T, bool Q8>
 int rms_device(Ctx* ctx, const RmsArgs& a, const void* X, const void* R, void* S, void* Y, void* Q, void* scales) {
+    constexpr int VEC = 16 / sizeof(T);
+    bool aligned = a.cols % VEC == 0 && a.ldx % VEC == 0 && (!R || a.ldr % VEC == 0) && a.rows < (int64_t(1) << 31);
+    for (const void* p : {X, R, static_cast<const void*>(S), static_cast<const void*>(Y), static_cast<const void*>(Q),
+                          static_cast<const void*>(a.gamma)})
+        aligned = aligned && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+    if (aligned) {
+        const int64_t packs = a.cols / VEC;
+        if (packs <= 32) return launch_rms<T, Q8, 32, 1>(ctx, a, X, R, S, Y, Q, scales);
+        if (packs <= 128) return launch_rms<T, Q8, 32, 4>(ctx, a, X, R, S, Y, Q, scales);
+        if (packs <= 512) return launch_rms<T, Q8, 128, 4>(ctx, a, X, R, S, Y, Q, scales);
+        if (packs <= 1024) return launch_rms<T, Q8, 256, 4>(ctx, a, X, R, S, Y, Q, scales);
+        if (packs <= 2048) return launch_rms<T, Q8, 512, 4>(ctx, a, X, R, S, Y, Q, scales);
+        if (packs <= 4096) return launch_rms<T, Q8, 1024, 4>(ctx, a, X, R, S, Y, Q, scales);
+    }
     const size_t smem = size_t(a.cols) * 4;
     auto kernel = rmsnorm_row_kernel<T, Q8>;
     if (smem > 48 * 1024) DOCC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));

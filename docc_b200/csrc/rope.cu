@@ -27,63 +27,129 @@ struct RopeTensor {
     int heads;
 };
 
-__device__ __forceinline__ void rope_angle(const RopeArgs& a, int64_t token, int i, float& c, float& s) {
-    const double turns = double(a.positions[token]) * (a.inv_freq[i] * 0.15915494309189533577);
-    float cs, sn;
-    sincospif(2.f * float(turns - rint(turns)), &sn, &cs);
-    c = a.mscale * cs;
-    s = a.mscale * a.sign * sn;
-}
-
-// Any strides and sizes: a block per token, an element pair (or one copied element) per thread and step.
-template <typename T>
+// Blocks (x, y): block x takes tokens, block y a share of the token's units. The token's cosines and sines are worked out once per
+// block, while the first unit of every thread is on its way, and serve all heads. A unit is VEC pairs, i.e. two runs of VEC
+// elements: VEC apart by rotary / 2 in the half layout, next to each other otherwise and in the part that is only copied.
+template <typename T, int VEC>
 __global__ void __launch_bounds__(256) rope_kernel(RopeTensor q, RopeTensor k, RopeTensor v, RopeArgs a) {
+    using P = Pack<T, VEC>;
+    extern __shared__ float2 turn_s[];  // cosine and sine of each pair, times mscale
+    __shared__ int64_t place_s[2];      // page (-1: nothing is written) and place of the token
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
-    const int half = int(a.rotary / 2), D = int(a.D), units = half + (D - int(a.rotary));
-    const int heads = q.heads + k.heads + v.heads;
+    const int half = int(a.rotary / 2), D = int(a.D), turned = half / VEC;
+    const int per_head = turned + (D - int(a.rotary) + 2 * VEC - 1) / (2 * VEC);
+    const int units = (q.heads + k.heads + v.heads) * per_head, step = 256 * gridDim.y;
+    const int first = int(blockIdx.y) * 256 + int(threadIdx.x);
     for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
-        const int64_t slot = a.slots ? a.slots[t] : 0;
-        const bool fits = !a.slots || (slot >= 0 && slot / a.page_size < a.num_pages);
-        if (!fits && slot >= 0 && threadIdx.x == 0) report_bad_index(a.status, kIndexSlot);
-        const int64_t page = a.slots ? slot / a.page_size : 0, place = a.slots ? slot % a.page_size : 0;
-        for (int w = threadIdx.x; w < heads * units; w += 256) {
-            int h = w / units;
-            const int u = w % units;
-            const RopeTensor* x = &q;
-            if (h >= q.heads) { h -= q.heads; x = &k; if (h >= k.heads) { h -= k.heads; x = &v; } }
-            const bool cached = x != &q;
-            if (cached && !fits) continue;
-            const T* in = static_cast<const T*>(x->in) + t * x->in_t + h * x->in_h;
-            T* out = static_cast<T*>(x->out) + (cached ? page * x->out_t + place * x->out_s : t * x->out_t) + h * x->out_h;
-            if (u >= half) {
-                const int d = int(a.rotary) + u - half;
-                out[d] = in[d];
-                continue;
+        P x0, x1;
+        const RopeTensor* of;
+        int h, u, d0, d1;
+        auto fetch = [&](int w) {
+            h = w / per_head;
+            u = w - h * per_head;
+            of = &q;
+            if (h >= q.heads) {
+                h -= q.heads;
+                of = &k;
+                if (h >= k.heads) {
+                    h -= k.heads;
+                    of = &v;
+                }
             }
-            const int d0 = a.interleaved ? 2 * u : u, d1 = a.interleaved ? 2 * u + 1 : u + half;
-            const T e0 = in[d0], e1 = in[d1];
-            if (x == &v) {
-                out[d0] = e0;
-                out[d1] = e1;
-                continue;
+            if (u >= turned) {
+                d0 = int(a.rotary) + (u - turned) * 2 * VEC;
+                d1 = d0 + VEC;
+            } else {
+                d0 = a.interleaved ? u * 2 * VEC : u * VEC;
+                d1 = a.interleaved ? d0 + VEC : d0 + half;
             }
+            const T* in = static_cast<const T*>(of->in) + t * of->in_t + h * of->in_h;
+            x0 = load_pack(reinterpret_cast<const P*>(in + d0));
+            if (VEC > 1 || d1 < D) x1 = load_pack(reinterpret_cast<const P*>(in + d1));
+        };
+        if (first < units) fetch(first);
+        for (int i = threadIdx.x; i < half; i += 256) {
+            const double turns = double(a.positions[t]) * (a.inv_freq[i] * 0.15915494309189533577);
             float c, s;
-            rope_angle(a, t, u, c, s);
-            const float x0 = to_float(e0), x1 = to_float(e1);
-            out[d0] = from_float<T>(x0 * c - x1 * s);
-            out[d1] = from_float<T>(x1 * c + x0 * s);
+            sincospif(2.f * float(turns - rint(turns)), &s, &c);
+            turn_s[i] = make_float2(a.mscale * c, a.mscale * a.sign * s);
         }
+        if (a.slots && threadIdx.x == 255) {
+            const int64_t slot = a.slots[t];
+            const int64_t page = slot < 0 ? -1 : slot / a.page_size;
+            if (page >= a.num_pages) report_bad_index(a.status, kIndexSlot);
+            place_s[0] = page < a.num_pages ? page : -1;
+            place_s[1] = slot - page * a.page_size;
+        }
+        __syncthreads();
+        for (int w = first; w < units; w += step) {
+            if (w != first) fetch(w);
+            const bool cached = of != &q;
+            if (cached && place_s[0] < 0) continue;
+            T* out = static_cast<T*>(of->out) + (cached ? place_s[0] * of->out_t + place_s[1] * of->out_s : t * of->out_t) + h * of->out_h;
+            if (u < turned && of != &v) {
+                if (a.interleaved) {
+#pragma unroll
+                    for (int e = 0; e < 2 * VEC; e += 2) {
+                        const float2 cs = turn_s[u * VEC + e / 2];
+                        T& e0 = e < VEC ? x0.v[e] : x1.v[e - VEC];
+                        T& e1 = e + 1 < VEC ? x0.v[e + 1 < VEC ? e + 1 : 0] : x1.v[e + 1 - VEC];
+                        const float f0 = to_float(e0), f1 = to_float(e1);
+                        e0 = from_float<T>(f0 * cs.x - f1 * cs.y);
+                        e1 = from_float<T>(f1 * cs.x + f0 * cs.y);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) {
+                        const float2 cs = turn_s[u * VEC + e];
+                        const float f0 = to_float(x0.v[e]), f1 = to_float(x1.v[e]);
+                        x0.v[e] = from_float<T>(f0 * cs.x - f1 * cs.y);
+                        x1.v[e] = from_float<T>(f1 * cs.x + f0 * cs.y);
+                    }
+                }
+            }
+            *reinterpret_cast<P*>(out + d0) = x0;
+            if (VEC > 1 || d1 < D) *reinterpret_cast<P*>(out + d1) = x1;
+        }
+        __syncthreads();  // turn_s and place_s are the next token's
     }
 }
 
-int rope_device(Ctx* ctx, int prec, const RopeTensor& q, const RopeTensor& k, const RopeTensor& v, const RopeArgs& a) {
-    const int64_t cap = int64_t(ctx->sm_count) * 8;
-    const dim3 grid(unsigned(a.tokens < cap ? a.tokens : cap));
-    if (prec == DOCC_B200_PREC_S) DOCC_CUDA_TRY(launch_pdl(rope_kernel<float>, grid, dim3(256), 0, ctx->stream, q, k, v, a));
-    else if (prec == DOCC_B200_PREC_H) DOCC_CUDA_TRY(launch_pdl(rope_kernel<__half>, grid, dim3(256), 0, ctx->stream, q, k, v, a));
-    else DOCC_CUDA_TRY(launch_pdl(rope_kernel<__nv_bfloat16>, grid, dim3(256), 0, ctx->stream, q, k, v, a));
+template <typename T, int VEC>
+int launch_rope(Ctx* ctx, const RopeTensor& q, const RopeTensor& k, const RopeTensor& v, const RopeArgs& a) {
+    const int64_t per_head = a.rotary / 2 / VEC + ceil_div(a.D - a.rotary, 2 * VEC);
+    const int64_t units = (int64_t(q.heads) + k.heads + v.heads) * per_head;
+    // few tokens: a unit per thread; many: a block per token, so that its angles are worked out once
+    const int64_t shares = ceil_div(units, 256);
+    const int64_t y = a.tokens * shares <= 2 * int64_t(ctx->sm_count) ? shares : 1;
+    const int64_t cap = int64_t(1) << 20;
+    const size_t smem = size_t(a.rotary / 2) * sizeof(float2);
+    DOCC_CUDA_TRY(launch_pdl(rope_kernel<T, VEC>, dim3(unsigned(a.tokens < cap ? a.tokens : cap), unsigned(y)), dim3(256), smem, ctx->stream, q, k,
+                             v, a));
     return after_launch(ctx, "rope_kernel");
+}
+
+template <typename T>
+int rope_typed(Ctx* ctx, const RopeTensor& q, const RopeTensor& k, const RopeTensor& v, const RopeArgs& a) {
+    auto fits = [&](int vec) {
+        bool ok = a.rotary / 2 % vec == 0 && (a.D - a.rotary) % (2 * vec) == 0;
+        for (const RopeTensor* x : {&q, &k, &v}) {
+            if (x->heads == 0) continue;
+            for (const void* p : {x->in, static_cast<const void*>(x->out)}) ok = ok && reinterpret_cast<uintptr_t>(p) % (vec * sizeof(T)) == 0;
+            for (int64_t s : {x->in_t, x->in_h, x->out_t, x->out_h, x->out_s}) ok = ok && s % vec == 0;
+        }
+        return ok;
+    };
+    constexpr int VEC = 16 / sizeof(T);
+    if (fits(VEC)) return launch_rope<T, VEC>(ctx, q, k, v, a);
+    if (fits(VEC / 2)) return launch_rope<T, VEC / 2>(ctx, q, k, v, a);
+    return launch_rope<T, 1>(ctx, q, k, v, a);
+}
+int rope_device(Ctx* ctx, int prec, const RopeTensor& q, const RopeTensor& k, const RopeTensor& v, const RopeArgs& a) {
+    if (prec == DOCC_B200_PREC_S) return rope_typed<float>(ctx, q, k, v, a);
+    if (prec == DOCC_B200_PREC_H) return rope_typed<__half>(ctx, q, k, v, a);
+    return rope_typed<__nv_bfloat16>(ctx, q, k, v, a);
 }
 
 int rope_check(const char* what, int prec, int64_t tokens, int64_t heads, int64_t D, int64_t rotary, const RopeArgs& a) {

@@ -356,33 +356,68 @@ def layernorm(X, gamma=None, beta=None, eps=1e-5, flags=0):
 
 
 # ---- the decoder step: RMS norm, rotary positions and the paged cache, attention over it, log-probabilities -----------------------
+# These calls are short on the device, so that what the host does around them is most of a step: the helpers ask a tensor for as
+# little as the checks need.
+_Pairs, _Triples = _i64 * 2, _i64 * 3
+
+
+def _addr(x):
+    """The address of an array of either side, or None."""
+    if x is None:
+        return None
+    try:
+        return x.data_ptr()
+    except AttributeError:
+        return x.ctypes.data
+
+
 def _side(*xs):
     """``_kind`` without its demand for contiguity, for entries that take strides: flags, after checking that all arrays live on the
     same side and, for torch tensors, on the device that the calling thread's launches go to."""
-    host = device = 0
+    host = device = False
     current = None
     for x in xs:
         if x is None:
             continue
         if _is_torch(x):
-            if not x.is_cuda:
-                raise TypeError("torch tensors must live on a CUDA device (pass numpy arrays for host data)")
-            if current is None:
-                import torch
+            at = x.get_device()
+            if at != current:
+                if at < 0:
+                    raise TypeError("torch tensors must live on a CUDA device (pass numpy arrays for host data)")
+                if current is None:
+                    import torch
 
-                current = torch.cuda.current_device()
-            if x.get_device() != current:
-                raise ValueError(f"tensor on cuda:{x.get_device()} while the calling thread's device is cuda:{current}")
-            device += 1
+                    current = torch.cuda.current_device()
+                if at != current:
+                    raise ValueError(f"tensor on cuda:{at} while the calling thread's device is cuda:{current}")
+            device = True
         elif isinstance(x, DeviceArray):
-            device += 1
+            device = True
         else:
             if not x.flags["C_CONTIGUOUS"]:
                 raise ValueError("arrays must be C-contiguous")
-            host += 1
+            host = True
     if host and device:
         raise TypeError("mix of host arrays and device tensors")
     return FLAG_HOST_PTRS if host else 0
+
+
+def _new_like(x):
+    """An uninitialised contiguous array of x's kind, shape and element type."""
+    if _is_torch(x) and x.is_contiguous():
+        import torch
+
+        return torch.empty_like(x)
+    return _new(x, x.shape)
+
+
+def _new(x, shape, name=None):
+    """An uninitialised contiguous array of x's kind, of element type ``name`` (None: x's own)."""
+    if _is_torch(x):
+        if name is None:
+            return x.new_empty(shape)
+        return x.new_empty(shape, dtype=_like(x, name))
+    return _empty(x, shape, None if name is None else np.dtype(name))
 
 
 def _heads_strides(x, name, written=False):
@@ -390,51 +425,58 @@ def _heads_strides(x, name, written=False):
     a broadcast view, whose elements share memory."""
     if not _is_torch(x) or x.is_contiguous():
         return None
-    s = x.stride()
-    if written and any(v == 0 and n > 1 for v, n in zip(s, x.shape)):
-        raise ValueError(f"{name}: a broadcast view cannot be written")
-    if s[-1] != 1 and x.shape[-1] > 1:
+    s, shape = x.stride(), x.shape
+    if s[-1] != 1 and shape[-1] > 1:
         raise ValueError(f"{name}: the last dimension must be contiguous")
-    if any(v < 0 for v in s):
-        raise ValueError(f"{name}: negative strides")
-    return _arr(s[:-1])
+    if written and 0 in s:
+        for d, v in enumerate(s):
+            if v == 0 and shape[d] > 1:
+                raise ValueError(f"{name}: a broadcast view cannot be written")
+    return _Pairs(s[0], s[1]) if len(s) == 3 else _Triples(s[0], s[1], s[2])
 
 
 def _rows_of(x, name):
     """(rows, cols, row stride) of a tensor seen as rows over its last dimension; the leading dimensions must be one strided run."""
-    cols = int(x.shape[-1])
-    rows = 1
-    for s in x.shape[:-1]:
-        rows *= int(s)
+    shape = x.shape
+    cols, rows = shape[-1], 1
+    for s in shape[:-1]:
+        rows *= s
     if not _is_torch(x) or x.is_contiguous():
         return rows, cols, cols
-    s = x.stride()
-    run = s[-2] if x.ndim > 1 else cols
-    step = run
+    s, run, step = x.stride(), None, None
     for d in range(x.ndim - 2, -1, -1):
-        if x.shape[d] != 1 and s[d] != step:
+        if shape[d] == 1:
+            continue
+        if run is None:
+            run = step = s[d]
+        if s[d] != step:
             raise ValueError(f"{name}: the leading dimensions are not one run of rows")
-        step *= x.shape[d]
-    if (s[-1] != 1 and cols > 1) or (run < cols and rows > 1):
+        step *= shape[d]
+    if (s[-1] != 1 and cols > 1) or (run is not None and run < cols):
         raise ValueError(f"{name}: rows must be contiguous and must not overlap")
-    return rows, cols, max(run, cols)
+    return rows, cols, cols if run is None else run
 
 
 def _want(x, dtype, name, shape=None):
     if _type_name(x.dtype) != dtype:
         raise TypeError(f"{name} must be {dtype}, not {_type_name(x.dtype)}")
-    if shape is not None and tuple(x.shape) != tuple(shape):
+    if shape is not None and x.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(x.shape)}")
     if _is_torch(x) and not x.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
 
 
+_torch_dtypes = {}
+
+
 def _like(x, name):
     """The element type ``name`` in the library ``x`` comes from."""
     if _is_torch(x):
-        import torch
+        if name not in _torch_dtypes:
+            import torch
 
-        return getattr(torch, name)
+            _torch_dtypes[name] = getattr(torch, name)
+        return _torch_dtypes[name]
     return np.dtype(name)
 
 
@@ -447,7 +489,7 @@ def _rms_inputs(X, gamma, residual, flags):
     if gamma is not None:
         _want(gamma, "float32", "rmsnorm: gamma", (cols,))
     if residual is not None:
-        if tuple(residual.shape) != tuple(X.shape) or _prec(residual) != _prec(X):
+        if residual.shape != X.shape or residual.dtype != X.dtype:
             raise ValueError("rmsnorm: the residual must have the shape and type of the input")
         ldr = _rows_of(residual, "rmsnorm: residual")[2]
     return rows, cols, ldx, ldr, flags
@@ -457,9 +499,9 @@ def rmsnorm(X, gamma=None, residual=None, eps=1e-6, flags=0):
     """``Y = s / sqrt(mean(s^2) + eps) * gamma`` over the last dimension, ``s = X + residual``. Returns Y, or with a residual
     ``(Y, S)``: S is s in the input's type, the residual of what follows. ``gamma`` is float32."""
     rows, cols, ldx, ldr, flags = _rms_inputs(X, gamma, residual, flags)
-    Y = _empty(X, X.shape)
-    S = _empty(X, X.shape) if residual is not None else None
-    call("docc_b200_rmsnorm", _prec(X), rows, cols, _ptr(X), ldx, _ptr(residual), ldr, _ptr(gamma), float(eps), _ptr(S), _ptr(Y), flags)
+    Y = _new_like(X)
+    S = _new_like(X) if residual is not None else None
+    call("docc_b200_rmsnorm", _prec(X), rows, cols, _addr(X), ldx, _addr(residual), ldr, _addr(gamma), eps, _addr(S), _addr(Y), flags)
     return Y if residual is None else (Y, S)
 
 
@@ -470,12 +512,11 @@ def rmsnorm_quant(X, gamma=None, residual=None, eps=1e-6, group=0, flags=0):
     rows, cols, ldx, ldr, flags = _rms_inputs(X, gamma, residual, flags)
     if group not in (0, 128):
         raise ValueError("rmsnorm_quant: group must be 0 (whole rows) or 128")
-    lead = tuple(X.shape[:-1])
-    Q = _empty(X, X.shape, _like(X, "float8_e4m3fn" if _is_torch(X) else "uint8"))
-    scales = _empty(X, lead + (1 if group == 0 else -(-cols // group),), _like(X, "float32"))
-    S = _empty(X, X.shape) if residual is not None else None
-    call("docc_b200_rmsnorm_q8", _prec(X), rows, cols, _ptr(X), ldx, _ptr(residual), ldr, _ptr(gamma), float(eps), int(group), _ptr(S),
-         _ptr(Q), _ptr(scales), flags)
+    Q = _new(X, X.shape, "float8_e4m3fn" if _is_torch(X) else "uint8")
+    scales = _new(X, tuple(X.shape[:-1]) + (1 if group == 0 else -(-cols // group),), "float32")
+    S = _new_like(X) if residual is not None else None
+    call("docc_b200_rmsnorm_q8", _prec(X), rows, cols, _addr(X), ldx, _addr(residual), ldr, _addr(gamma), eps, group, _addr(S), _addr(Q),
+         _addr(scales), flags)
     return (Q, scales) if residual is None else (Q, scales, S)
 
 
@@ -511,6 +552,21 @@ def rope_frequencies(rotary_dim, base=10000.0, scaling="none", factor=1.0, origi
     return freq / factor * stretched + freq * (1.0 - stretched), 0.1 * math.log(factor) + 1.0
 
 
+def _rope_inputs(x, positions, inv_freq, name):
+    _want(positions, "int64", f"{name}: positions", (x.shape[0],))
+    _want(inv_freq, "float64", f"{name}: inv_freq")
+    if inv_freq.ndim != 1 or 2 * inv_freq.shape[0] > x.shape[2]:
+        raise ValueError(f"{name}: inv_freq must hold one frequency per pair, at most D / 2")
+
+
+def _out_like(x, out, name):
+    if out is None:
+        return _new_like(x)
+    if out.shape != x.shape or out.dtype != x.dtype:
+        raise ValueError(f"{name}: out must have the shape and type of the query")
+    return out
+
+
 def rope(X, positions, inv_freq, interleaved=False, mscale=1.0, inverse=False, out=None, flags=0):
     """Rotary positions on X [tokens, heads, D] (``docc_b200_rope``): ``positions`` int64 [tokens], ``inv_freq`` float64
     [rotary_dim / 2] on the side of X (``rope_frequencies``). ``inverse`` applies the transpose, which is the gradient. ``out`` may be
@@ -519,29 +575,21 @@ def rope(X, positions, inv_freq, interleaved=False, mscale=1.0, inverse=False, o
     if X.ndim != 3:
         raise ValueError("rope: X must be [tokens, heads, D]")
     T, H, D = X.shape
-    _want(positions, "int64", "rope: positions", (T,))
-    _want(inv_freq, "float64", "rope: inv_freq")
-    if inv_freq.ndim != 1 or 2 * inv_freq.shape[0] > D:
-        raise ValueError("rope: inv_freq must hold one frequency per pair, at most D / 2")
-    if out is None:
-        out = _empty(X, X.shape)
-    elif tuple(out.shape) != tuple(X.shape) or _prec(out) != _prec(X):
-        raise ValueError("rope: out must have the shape and type of X")
-    xs, ys = _heads_strides(X, "rope: X"), _heads_strides(out, "rope: out", True)
-    call("docc_b200_rope", _prec(X), T, H, D, 2 * inv_freq.shape[0], int(bool(interleaved)), int(bool(inverse)), _ptr(X), xs,
-         _ptr(positions), _ptr(inv_freq), float(mscale), _ptr(out), ys, flags)
+    _rope_inputs(X, positions, inv_freq, "rope")
+    out = _out_like(X, out, "rope")
+    call("docc_b200_rope", _prec(X), T, H, D, 2 * inv_freq.shape[0], 1 if interleaved else 0, 1 if inverse else 0, _addr(X),
+         _heads_strides(X, "rope: X"), _addr(positions), _addr(inv_freq), mscale, _addr(out), _heads_strides(out, "rope: out", True), flags)
     return out
 
 
-def _cache(k_cache, v_cache, Hkv, D, prec, name):
+def _cache(q, k_cache, v_cache, Hkv, D, name):
     """(pages, page_size, strides of K, strides of V) of a cache [pages, Hkv, page_size, D] (views of other layouts included)."""
-    for c in (k_cache, v_cache):
-        if c.ndim != 4 or c.shape[1] != Hkv or c.shape[3] != D or _prec(c) != prec:
-            raise ValueError(f"{name}: caches must be [pages, {Hkv}, page_size, {D}] of the type of the query")
-    if tuple(k_cache.shape) != tuple(v_cache.shape):
+    shape = k_cache.shape
+    if v_cache.shape != shape:
         raise ValueError(f"{name}: the two caches differ in shape")
-    return (int(k_cache.shape[0]), int(k_cache.shape[2]), _heads_strides(k_cache, f"{name}: k_cache", True),
-            _heads_strides(v_cache, f"{name}: v_cache", True))
+    if len(shape) != 4 or shape[1] != Hkv or shape[3] != D or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise ValueError(f"{name}: caches must be [pages, {Hkv}, page_size, {D}] of the type of the query")
+    return shape[0], shape[2], _heads_strides(k_cache, f"{name}: k_cache", True), _heads_strides(v_cache, f"{name}: v_cache", True)
 
 
 def rope_append(q, k, v, positions, inv_freq, k_cache, v_cache, slots, interleaved=False, mscale=1.0, out=None, flags=0):
@@ -550,27 +598,24 @@ def rope_append(q, k, v, positions, inv_freq, k_cache, v_cache, slots, interleav
     (``out``, which may be q itself). Device tensors only; the slots of one call must differ."""
     if _side(q, k, v, positions, inv_freq, k_cache, v_cache, slots, out):
         raise TypeError("rope_append: the cache lives on the device; host arrays are not taken")
-    if q.ndim != 3 or k.ndim != 3 or tuple(k.shape) != tuple(v.shape) or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+    if q.ndim != 3 or k.ndim != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
         raise ValueError("rope_append: q must be [tokens, Hq, D], k and v [tokens, Hkv, D]")
     T, Hq, D = q.shape
-    Hkv, prec = k.shape[1], _prec(q)
-    if _prec(k) != prec or _prec(v) != prec:
+    Hkv = k.shape[1]
+    if k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError("rope_append: q, k and v differ in type")
-    _want(positions, "int64", "rope_append: positions", (T,))
+    _rope_inputs(q, positions, inv_freq, "rope_append")
     _want(slots, "int64", "rope_append: slots", (T,))
-    _want(inv_freq, "float64", "rope_append: inv_freq")
-    if inv_freq.ndim != 1 or 2 * inv_freq.shape[0] > D:
-        raise ValueError("rope_append: inv_freq must hold one frequency per pair, at most D / 2")
-    pages, page_size, ks, vs = _cache(k_cache, v_cache, Hkv, D, prec, "rope_append")
-    if out is None:
-        out = _empty(q, q.shape)
-    elif tuple(out.shape) != tuple(q.shape) or _prec(out) != prec:
-        raise ValueError("rope_append: out must have the shape and type of q")
-    call("docc_b200_rope_append", prec, T, Hq, Hkv, D, 2 * inv_freq.shape[0], int(bool(interleaved)), _ptr(q),
-         _heads_strides(q, "rope_append: q"), _ptr(k), _heads_strides(k, "rope_append: k"), _ptr(v), _heads_strides(v, "rope_append: v"),
-         _ptr(positions), _ptr(inv_freq), float(mscale), _ptr(out), _heads_strides(out, "rope_append: out", True), _ptr(k_cache), ks,
-         _ptr(v_cache), vs, pages, page_size, _ptr(slots), flags)
+    pages, page_size, ks, vs = _cache(q, k_cache, v_cache, Hkv, D, "rope_append")
+    out = _out_like(q, out, "rope_append")
+    call("docc_b200_rope_append", _prec(q), T, Hq, Hkv, D, 2 * inv_freq.shape[0], 1 if interleaved else 0, _addr(q),
+         _heads_strides(q, "rope_append: q"), _addr(k), _heads_strides(k, "rope_append: k"), _addr(v), _heads_strides(v, "rope_append: v"),
+         _addr(positions), _addr(inv_freq), mscale, _addr(out), _heads_strides(out, "rope_append: out", True), _addr(k_cache), ks,
+         _addr(v_cache), vs, pages, page_size, _addr(slots), flags)
     return out
+
+
+_scratch_bytes = {}  # (device, query heads per key-value head, D) -> bytes: what the size of the scratch depends on
 
 
 def paged_attention(q, k_cache, v_cache, page_table, lengths, scale=None, softcap=0.0, window=0, return_lse=False, out=None, flags=0):
@@ -583,29 +628,32 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, scale=None, softca
     With torch tensors the scratch comes from torch's allocator, so a captured graph owns the scratch it replays with."""
     if _side(q, k_cache, v_cache, page_table, lengths, out):
         raise TypeError("paged_attention: the cache lives on the device; host arrays are not taken")
-    if q.ndim != 3:
-        raise ValueError("paged_attention: q must be [B, Hq, D]")
+    if q.ndim != 3 or k_cache.ndim != 4:
+        raise ValueError("paged_attention: q must be [B, Hq, D] and the caches [pages, Hkv, page_size, D]")
     B, Hq, D = q.shape
     Hkv, prec = k_cache.shape[1], _prec(q)
-    pages, page_size, ks, vs = _cache(k_cache, v_cache, Hkv, D, prec, "paged_attention")
+    pages, page_size, ks, vs = _cache(q, k_cache, v_cache, Hkv, D, "paged_attention")
     if Hkv == 0 or Hq % Hkv:
         raise ValueError(f"paged_attention: {Hq} query heads are not a multiple of {Hkv} key-value heads")
     _want(lengths, "int32", "paged_attention: lengths", (B,))
     if page_table.ndim != 2:
         raise ValueError("paged_attention: page_table must be [B, max_pages]")
-    _want(page_table, "int32", "paged_attention: page_table", (B, page_table.shape[1]))
-    if out is None:
-        out = _empty(q, q.shape)
-    elif tuple(out.shape) != tuple(q.shape) or _prec(out) != prec:
-        raise ValueError("paged_attention: out must have the shape and type of q")
-    lse = _empty(q, (B, Hq), _like(q, "float32")) if return_lse else None
-    bytes_ = _lib._sz()
-    call("docc_b200_paged_attention_workspace", prec, B, Hq, Hkv, D, ctypes.byref(bytes_))
-    work = _empty(q, (bytes_.value,), _like(q, "uint8")) if bytes_.value and _is_torch(q) else None
-    call("docc_b200_paged_attention", prec, B, Hq, Hkv, D, 1.0 / math.sqrt(max(D, 1)) if scale is None else float(scale), float(softcap),
-         int(window), _ptr(q), _heads_strides(q, "paged_attention: q"), _ptr(k_cache), ks, _ptr(v_cache), vs, pages, page_size,
-         _ptr(page_table), page_table.shape[1], page_table.shape[1], _ptr(lengths), _ptr(out),
-         _heads_strides(out, "paged_attention: out", True), _ptr(lse), _ptr(work), bytes_.value if work is not None else 0, flags)
+    most = page_table.shape[1]
+    _want(page_table, "int32", "paged_attention: page_table", (B, most))
+    out = _out_like(q, out, "paged_attention")
+    lse = _new(q, (B, Hq), "float32") if return_lse else None
+    work, bytes_ = None, 0
+    if _is_torch(q):
+        key = (q.get_device(), Hq // Hkv, D)
+        bytes_ = _scratch_bytes.get(key)
+        if bytes_ is None:
+            size = ctypes.c_size_t()
+            call("docc_b200_paged_attention_workspace", prec, 1, Hq, Hkv, D, ctypes.byref(size))
+            bytes_ = _scratch_bytes[key] = size.value
+        work = _new(q, bytes_, "uint8")
+    call("docc_b200_paged_attention", prec, B, Hq, Hkv, D, 1.0 / math.sqrt(max(D, 1)) if scale is None else scale, softcap, window,
+         _addr(q), _heads_strides(q, "paged_attention: q"), _addr(k_cache), ks, _addr(v_cache), vs, pages, page_size, _addr(page_table),
+         most, most, _addr(lengths), _addr(out), _heads_strides(out, "paged_attention: out", True), _addr(lse), _addr(work), bytes_, flags)
     return (out, lse) if return_lse else out
 
 
@@ -618,11 +666,10 @@ def token_logprobs(logits, ids, k=0, scale=1.0, flags=0):
         raise ValueError("token_logprobs: logits must be [rows, vocab]")
     rows, vocab, ldx = _rows_of(logits, "token_logprobs")
     _want(ids, "int64", "token_logprobs: ids", (rows,))
-    f32, i64 = _like(logits, "float32"), _like(logits, "int64")
-    logp, entropy = _empty(logits, (rows,), f32), _empty(logits, (rows,), f32)
-    top_ids, top_logp = _empty(logits, (rows, k), i64), _empty(logits, (rows, k), f32)
-    call("docc_b200_token_logprobs", _prec(logits), rows, vocab, _ptr(logits), ldx, float(scale), _ptr(ids), _ptr(logp), _ptr(entropy),
-         int(k), _ptr(top_ids), _ptr(top_logp), flags)
+    logp, entropy = _new(logits, (rows,), "float32"), _new(logits, (rows,), "float32")
+    top_ids, top_logp = _new(ids, (rows, k)), _new(logits, (rows, k), "float32")
+    call("docc_b200_token_logprobs", _prec(logits), rows, vocab, _addr(logits), ldx, scale, _addr(ids), _addr(logp), _addr(entropy), k,
+         _addr(top_ids), _addr(top_logp), flags)
     return logp, entropy, top_ids, top_logp
 
 
