@@ -28,17 +28,27 @@ __device__ __forceinline__ float warp_max_nan(float v) {
     for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
-// y / scale with the division rounded once: a product with the rounded reciprocal would move values that lie next to the
-// middle of two codes to the other one.
-__device__ __forceinline__ uint8_t quantise(float y, float scale) {
-    return __nv_cvt_float_to_fp8(scale == 0.f ? 0.f : __fdiv_rn(y, scale), __NV_SATFINITE, __NV_E4M3);
-}
+// What turns a group's values into codes: q = e4m3((y lift) inv), inv = 448 / (max|y| lift). A product in place of the division by
+// the scale moves a value by 2 steps of fp32 at most, less than the norm itself is off. lift keeps the reciprocal of a tiny maximum
+// finite. A group of zeros has inv 0, a group with a NaN inv NaN.
+struct Quantiser {
+    float lift, inv, scale;
+    __device__ __forceinline__ explicit Quantiser(float top) {
+        lift = top < 0x1p-96f ? 0x1p96f : 1.f;
+        inv = top == 0.f ? 0.f : __fdiv_rn(kE4m3Max, top * lift);
+        scale = __fdiv_rn(top, kE4m3Max);
+    }
+    __device__ __forceinline__ uint16_t two(float a, float b) const {
+        return __nv_cvt_float2_to_fp8x2(make_float2(a * lift * inv, b * lift * inv), __NV_SATFINITE, __NV_E4M3);
+    }
+    __device__ __forceinline__ uint8_t one(float a) const { return uint8_t(two(a, 0.f)); }
+};
 
-template <int N> __device__ __forceinline__ void store_codes(uint8_t* q, const float (&y)[N], float scale) {
-    Pack<uint8_t, N> c;  // N-byte aligned: cols and the row's first code are multiples of N
+template <int N> __device__ __forceinline__ void store_codes(uint8_t* q, const float (&y)[N], const Quantiser& by) {
+    Pack<uint16_t, N / 2> c;  // N-byte aligned: cols and the row's first code are multiples of N
 #pragma unroll
-    for (int e = 0; e < N; e++) c.v[e] = quantise(y[e], scale);
-    *reinterpret_cast<Pack<uint8_t, N>*>(q) = c;
+    for (int e = 0; e < N; e += 2) c.v[e / 2] = by.two(y[e], y[e + 1]);
+    *reinterpret_cast<Pack<uint16_t, N / 2>*>(q) = c;
 }
 
 struct RmsArgs {
@@ -135,10 +145,10 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) rmsnorm_kernel(const T*
                 top = 0.f;
 #pragma unroll
                 for (int o = LANES / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-                const float scale = __fdiv_rn(m, kE4m3Max);
+                const Quantiser by(m);
                 if (ok && p < packs) {
-                    store_codes<VEC>(Q + row * a.cols + int64_t(p) * VEC, v[i], scale);
-                    if (lane % LANES == 0) scales[row * ((a.cols + kRmsGroup - 1) / kRmsGroup) + p / LANES] = scale;
+                    store_codes<VEC>(Q + row * a.cols + int64_t(p) * VEC, v[i], by);
+                    if (lane % LANES == 0) scales[row * ((a.cols + kRmsGroup - 1) / kRmsGroup) + p / LANES] = by.scale;
                 }
             }
         }
@@ -153,13 +163,13 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) rmsnorm_kernel(const T*
 #pragma unroll
                 for (int w = 1; w < WPR; w++) top = max_nan(top, red[1][rib][w]);
             }
-            const float scale = __fdiv_rn(top, kE4m3Max);
+            const Quantiser by(top);
 #pragma unroll
             for (int i = 0; i < VPT; i++) {
                 const int p = i * TPR + t;
-                if (ok && p < packs) store_codes<VEC>(Q + row * a.cols + int64_t(p) * VEC, v[i], scale);
+                if (ok && p < packs) store_codes<VEC>(Q + row * a.cols + int64_t(p) * VEC, v[i], by);
             }
-            if (ok && t == 0) scales[row] = scale;
+            if (ok && t == 0) scales[row] = by.scale;
         }
     }
 }
@@ -207,9 +217,9 @@ __global__ void __launch_bounds__(256) rmsnorm_row_kernel(const T* X, const T* R
                 __syncthreads();
                 m = red[0];
                 for (int w = 1; w < 8; w++) m = max_nan(m, red[w]);
-                const float scale = __fdiv_rn(m, kE4m3Max);
-                for (int c = t; c < cols; c += 256) Q[row * a.cols + c] = quantise(row_s[c], scale);
-                if (t == 0) scales[row] = scale;
+                const Quantiser by(m);
+                for (int c = t; c < cols; c += 256) Q[row * a.cols + c] = by.one(row_s[c]);
+                if (t == 0) scales[row] = by.scale;
             } else {
                 for (int g = warp; g < groups; g += 8) {
                     const int c0 = int(g * a.group), c1 = int(c0 + a.group < a.cols ? c0 + a.group : a.cols);
@@ -221,13 +231,13 @@ __global__ void __launch_bounds__(256) rmsnorm_row_kernel(const T* X, const T* R
                         if (c < c1) y[i] = a.gamma ? row_s[c] * rstd * a.gamma[c] : row_s[c] * rstd;
                         m = max_nan(m, fabsf(y[i]));
                     }
-                    const float scale = __fdiv_rn(warp_max_nan(m), kE4m3Max);
+                    const Quantiser by(warp_max_nan(m));
 #pragma unroll
                     for (int i = 0; i < kRmsGroup / 32; i++) {
                         const int c = c0 + lane + 32 * i;
-                        if (c < c1) Q[row * a.cols + c] = quantise(y[i], scale);
+                        if (c < c1) Q[row * a.cols + c] = by.one(y[i]);
                     }
-                    if (lane == 0) scales[row * groups + g] = scale;
+                    if (lane == 0) scales[row * groups + g] = by.scale;
                 }
             }
         }
