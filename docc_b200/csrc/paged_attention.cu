@@ -26,6 +26,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
+constexpr int kRowCost = 1;
 constexpr int64_t kMostTokens = (int64_t(1) << 31) - 4096;  // token numbers of a chunk past the end still fit in 32 bits
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -63,56 +64,70 @@ __device__ __forceinline__ void visible(const PagedArgs& a, int b, int& lo, int&
 // An empty sequence has one chunk without visible keys, so that its output is written like any other.
 __device__ __forceinline__ int chunks_of(const PagedArgs& a, int lo, int n) { return n > lo ? (n - lo + a.chunk - 1) / a.chunk : 1; }
 
-// A place on the line of chunks: sequence-major, then key-value head, then tile of query heads, then chunk.
+// A place on the line of chunks: sequence-major, then key-value head, then tile of query heads, then chunk. Every row also counts
+// kRowCost chunks in front of its first that hold nothing: they stand for the merge and the new queries, without which a run of
+// many short rows takes far longer than a run of one long row.
 struct Cursor {
     int b, kvh, tile, chunk, chunks, lo, n;
+    int64_t left;  // what is left of the run on the line, this chunk included
     __device__ __forceinline__ void enter(const PagedArgs& a) {
         visible(a, b, lo, n);
         chunks = chunks_of(a, lo, n);
     }
-    __device__ __forceinline__ void next(const PagedArgs& a) {
-        if (++chunk < chunks) return;
+    // to the run's next chunk; false if there is none
+    __device__ __forceinline__ bool next(const PagedArgs& a) {
+        if (--left <= 0) return false;
+        if (++chunk < chunks) return true;
+        left -= kRowCost;
+        if (left <= 0) return false;
         chunk = 0;
-        if (++tile < a.tiles) return;
+        if (++tile < a.tiles) return true;
         tile = 0;
-        if (++kvh < a.Hkv) return;
+        if (++kvh < a.Hkv) return true;
         kvh = 0;
-        if (++b < a.B) enter(a);
+        b++;
+        enter(a);
+        return true;
     }
 };
 
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {  // both positive; 32 bits where they fit
+    return ((a | b) >> 32) == 0 ? int64_t(uint32_t(a) / uint32_t(b)) : a / b;
+}
+
 struct Run {
-    int64_t begin, end, total;
-    int blocks;  // runs in all: never more than there are chunks, so that none is empty
+    int64_t begin, end, base, extra;  // the first `extra` runs are base + 1 long, the others base
     Cursor at;
+    __device__ __forceinline__ int block_of(int64_t place) const {
+        const int64_t longer = extra * (base + 1);
+        return int(place < longer ? divide(place, base + 1) : extra + divide(place - longer, base));
+    }
 };
 
-// The calling warp's run and its first chunk. Every warp works it out for itself, 32 sequences at a time.
+// The calling warp's run and its first chunk; false if the run holds none. Every warp works it out for itself, 32 sequences at a time.
 __device__ __forceinline__ bool find_run(const PagedArgs& a, Run& r) {
     const int lane = threadIdx.x & 31;
     const int64_t rows = int64_t(a.Hkv) * a.tiles;
-    int64_t sum = 0;
-    for (int b = lane; b < a.B; b += 32) {
+    auto length_of = [&](int b) -> int64_t {  // of a sequence's rows on the line
+        if (b >= a.B) return 0;
         int lo, n;
         visible(a, b, lo, n);
-        sum += chunks_of(a, lo, n);
-    }
+        return (chunks_of(a, lo, n) + kRowCost) * rows;
+    };
+    const int64_t first = length_of(lane);
+    int64_t total = first;
+    for (int b = lane + 32; b < a.B; b += 32) total += length_of(b);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    r.total = sum * rows;
-    r.blocks = r.total < int64_t(gridDim.x) ? int(r.total) : int(gridDim.x);
-    if (int(blockIdx.x) >= r.blocks) return false;
-    r.begin = int64_t(blockIdx.x) * r.total / r.blocks;
-    r.end = (int64_t(blockIdx.x) + 1) * r.total / r.blocks;
-    int64_t before = 0;  // chunks of the sequences before this group of 32, times rows
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    r.base = divide(total, gridDim.x);
+    r.extra = total - r.base * gridDim.x;
+    const int64_t c = blockIdx.x;
+    r.begin = c * r.base + (c < r.extra ? c : r.extra);
+    r.end = r.begin + r.base + (c < r.extra ? 1 : 0);
+    if (r.begin == r.end) return false;
+    int64_t before = 0;
     for (int base = 0; base < a.B; base += 32) {
-        const int b = base + lane;
-        int lo = 0, n = 0;
-        int64_t mine = 0;
-        if (b < a.B) {
-            visible(a, b, lo, n);
-            mine = chunks_of(a, lo, n) * rows;
-        }
+        const int64_t mine = base == 0 ? first : length_of(base + lane);
         int64_t upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -125,15 +140,17 @@ __device__ __forceinline__ bool find_run(const PagedArgs& a, Run& r) {
             const int64_t offset = r.begin - before - __shfl_sync(0xffffffffu, upto - mine, src);
             r.at.b = base + src;
             r.at.enter(a);
-            const int64_t row = offset / r.at.chunks;
-            r.at.chunk = int(offset % r.at.chunks);
-            r.at.kvh = int(row / a.tiles);
-            r.at.tile = int(row % a.tiles);
-            return true;
+            const int length = r.at.chunks + kRowCost, row = int(divide(offset, length));
+            const int place = int(offset - int64_t(row) * length);
+            r.at.chunk = place < kRowCost ? 0 : place - kRowCost;
+            r.at.left = r.end - r.begin - (place < kRowCost ? kRowCost - place : 0);
+            r.at.kvh = row / a.tiles;
+            r.at.tile = row - r.at.kvh * a.tiles;
+            return r.at.left > 0;
         }
         before += __shfl_sync(0xffffffffu, upto, 31);
     }
-    return false;  // not reached: begin < total
+    return false;  // not reached: begin lies on the line
 }
 __device__ __forceinline__ int row_of(const PagedArgs& a, const Cursor& c) { return (c.b * a.Hkv + c.kvh) * a.tiles + c.tile; }
 
@@ -165,6 +182,31 @@ __device__ __forceinline__ float score_log2(const PagedArgs& a, float dot) {
     const float s = dot * a.scale;
     return (a.softcap > 0.f ? a.softcap * tanhf(s / a.softcap) : s) * kLog2e;
 }
+// tanh y = 1 - 2 / (e^2y + 1) with an error of 4 * 2^-24 whatever y, against tanhf's 2^-23 relative one: softcap times that lies far
+// below what 16-bit keys leave of a score, and tanhf's two branches took half of the kernel's time. `turn` is 2 log2 e scale / softcap.
+__device__ __forceinline__ float capped_log2(float dot, float turn, float cap_log2e) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(ex2(dot * turn) + 1.f));
+    return fmaf(-2.f * cap_log2e, r, cap_log2e);
+}
+
+// The four warps' maxima and sums of one query head, and what each warp's output counts in the row's.
+struct Merged {
+    float top, sum, weight[kWarps];
+    template <typename Rows> __device__ __forceinline__ Merged(const Rows& ml, int row) {
+        top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) top = fmaxf(top, ml[w][row].x);
+        const float ref = top == -INFINITY ? 0.f : top;
+        sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+            weight[w] = ex2(ml[w][row].x - ref);
+            sum = fmaf(weight[w], ml[w][row].y, sum);
+        }
+    }
+    __device__ __forceinline__ float lse() const { return sum == 0.f ? -INFINITY : top * kLn2 + logf(sum); }
+};
 
 // ---- 16-bit inputs: tensor cores ---------------------------------------------------------------------------------------------
 // A warp step is 16 keys. S = Q K^T and O += P V run as m16n8k16 products with the (up to 16) query heads of the tile as rows: one
@@ -212,8 +254,9 @@ template <int DP> struct TcShape {
     static constexpr int kRow = DP * 2;                      // bytes of a key or value in shared memory
     static constexpr int kStage = 2 * 16 * kRow;             // 16 keys and 16 values of one warp
     static constexpr int kStages = DP <= 64 ? 5 : DP <= 96 ? 4 : 3;
-    static constexpr int kMerge = 16 * DP * 4;               // a warp's output, two of which are staged
-    static constexpr int kBytes = kWarps * kStages * kStage + 2 * kMerge;
+    static constexpr int kBytes = kWarps * kStages * kStage + kWarps * 8 * DP * 4;
+    // place of a pair of columns in a warp's eight merged rows: four rows at one column lie in different banks
+    static __device__ __forceinline__ int merged(int warp, int row, int d) { return (warp * 8 + row) * DP + (d ^ ((row & 3) << 3)); }
     // 16-byte pieces of a row are permuted so that the eight rows an ldmatrix reads at one column lie in different banks
     static __device__ __forceinline__ uint32_t offset(int row, int piece) {
         const int turn = DP == 96 ? (row >> 1) & 3 : row & 7;
@@ -221,7 +264,8 @@ template <int DP> struct TcShape {
     }
 };
 
-template <typename T, int DP>
+// HALVES: 1 where the tile has at most eight query heads (rows 8-15 of the fragments are padding), else 2.
+template <typename T, int DP, int HALVES>
 __global__ void __launch_bounds__(kThreads) paged_tc_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
                                                             T* __restrict__ O, PagedArgs a) {
     using Shape = TcShape<DP>;
@@ -246,8 +290,8 @@ __global__ void __launch_bounds__(kThreads) paged_tc_kernel(const T* __restrict_
         if (threadIdx.x == 0) a.begun[blockIdx.x] = make_int4(-1, 0, 0, 0);
         return;
     }
-    const int units = int(run.end - run.begin);
     Cursor load = run.at, at = run.at;
+    bool more = true;  // the load cursor stands on a chunk that has not been asked for
 
     const int key_lane = warp * 16 + (lane & 15);
     int key = load.lo + load.chunk * a.chunk + key_lane;
@@ -276,28 +320,28 @@ __global__ void __launch_bounds__(kThreads) paged_tc_kernel(const T* __restrict_
         cp_async_commit();
     };
     auto advance = [&]() {  // the entry is fetched one step before its copies are issued
-        load.next(a);
-        if (load.b < a.B) {
+        more = load.next(a);
+        if (more) {
             key = load.lo + load.chunk * a.chunk + key_lane;
             entry = page_entry(a, load, key);
         }
     };
-    int loaded = 0;
 #pragma unroll
     for (int s = 0; s < S - 1; s++) {
-        if (loaded < units) {
+        if (more) {
             issue(s);
-            if (++loaded < units) advance();
+            advance();
         } else {
             cp_async_commit();
         }
     }
 
+    const float scale_log2e = a.scale * kLog2e, turn = a.softcap > 0.f ? 2.f * scale_log2e / a.softcap : 0.f, cap_log2e = a.softcap * kLog2e;
     uint32_t qf[DP / 16][4];
-    float acc[NT][4], m[2], l[2];
-    int first_chunk = 0;
-    for (int u = 0; u < units; u++) {
-        if (u == 0 || at.chunk == 0) {  // a row begins
+    float acc[NT][4], m[HALVES], l[HALVES];
+    int first_chunk = -1, begun = -1, last = 0, stage = 0;
+    do {
+        if (first_chunk < 0) {  // a row begins
             first_chunk = at.chunk;
             const int r0 = at.tile * 16 + (lane >> 2);
             const T* q0 = Q + at.b * a.qs[0] + (int64_t(at.kvh) * a.group + r0) * a.qs[1];
@@ -309,25 +353,27 @@ __global__ void __launch_bounds__(kThreads) paged_tc_kernel(const T* __restrict_
                     const int d = kk * 16 + half * 8 + (lane & 3) * 2;
                     const bool in = d < a.D;
                     qf[kk][half * 2] = in && r0 < a.group ? *reinterpret_cast<const uint32_t*>(q0 + d) : 0u;
-                    qf[kk][half * 2 + 1] = in && r0 + 8 < a.group ? *reinterpret_cast<const uint32_t*>(q1 + d) : 0u;
+                    qf[kk][half * 2 + 1] = HALVES == 2 && in && r0 + 8 < a.group ? *reinterpret_cast<const uint32_t*>(q1 + d) : 0u;
                 }
             }
 #pragma unroll
             for (int i = 0; i < NT; i++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) acc[i][e] = 0.f;
-            m[0] = m[1] = -INFINITY;
-            l[0] = l[1] = 0.f;
+#pragma unroll
+            for (int r = 0; r < HALVES; r++) {
+                m[r] = -INFINITY;
+                l[r] = 0.f;
+            }
         }
         cp_async_wait<S - 2>();
         __syncwarp();  // every lane's copies of this step have landed, and every lane is done with the stage filled next
-        if (loaded < units) {
-            issue((u + S - 1) % S);
-            if (++loaded < units) advance();
+        if (more) {
+            issue(stage == 0 ? S - 1 : stage - 1);
+            advance();
         } else {
             cp_async_commit();
         }
-        const int stage = u % S;
         const uint32_t mask = mask_s[warp][stage];
         if (mask) {
             const uint32_t kb = ring_u + stage * Shape::kStage, vb = kb + 16 * Shape::kRow;
@@ -339,40 +385,56 @@ __global__ void __launch_bounds__(kThreads) paged_tc_kernel(const T* __restrict_
                 mma16816<T>(s[0], qf[kk], b[0], b[1]);
                 mma16816<T>(s[1], qf[kk], b[2], b[3]);
             }
+            if (a.softcap > 0.f) {
 #pragma unroll
-            for (int t = 0; t < 2; t++)
+                for (int t = 0; t < 2; t++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) s[t][e] = score_log2(a, s[t][e]);
+                    for (int e = 0; e < 2 * HALVES; e++) s[t][e] = capped_log2(s[t][e], turn, cap_log2e);
+            } else {
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int e = 0; e < 2 * HALVES; e++) s[t][e] *= scale_log2e;
+            }
             if (mask != 0xffffu) {
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
+                    for (int e = 0; e < 2 * HALVES; e++)
                         if (!((mask >> (t * 8 + (lane & 3) * 2 + (e & 1))) & 1)) s[t][e] = -INFINITY;
             }
-            float corr[2], ref[2];
+            float corr[HALVES], ref[HALVES];
+            bool moved = false;
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
+            for (int r = 0; r < HALVES; r++) {
                 float x = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
                 const float mn = fmaxf(m[r], x);
                 ref[r] = mn == -INFINITY ? 0.f : mn;  // only scores of -inf so far: 2^(-inf - 0) = 0, not a NaN
                 corr[r] = ex2(m[r] - ref[r]);
+                moved = moved || m[r] != mn;
                 m[r] = mn;
             }
-            if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
+            if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-                for (int i = 0; i < NT; i++)
+                for (int r = 0; r < HALVES; r++) {
+                    l[r] *= corr[r];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) acc[i][e] *= corr[e >> 1];
-                l[0] *= corr[0];
-                l[1] *= corr[1];
+                    for (int i = 0; i < NT; i++) {
+                        acc[i][2 * r] *= corr[r];
+                        acc[i][2 * r + 1] *= corr[r];
+                    }
+                }
             }
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
+                    if (e >= 2 * HALVES) {
+                        s[t][e] = 0.f;
+                        continue;
+                    }
                     s[t][e] = ex2(s[t][e] - ref[e >> 1]);
                     l[e >> 1] += s[t][e];
                 }
@@ -392,94 +454,56 @@ __global__ void __launch_bounds__(kThreads) paged_tc_kernel(const T* __restrict_
                 mma16816<T>(acc[2 * i + 1], lo, b[2], b[3]);
             }
         }
-        if (at.chunk + 1 == at.chunks || u + 1 == units) {  // the row, or this block's part of it, is complete
+        const bool row_done = at.chunk + 1 == at.chunks;
+        if (row_done || at.left == 1) {  // the row, or this block's part of it, is complete
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
+            for (int r = 0; r < HALVES; r++) {
                 l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
                 l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+                if ((lane & 3) == 0) ml_s[warp][(lane >> 2) + 8 * r] = make_float2(m[r], l[r]);
             }
-            if ((lane & 3) == 0) {
-                ml_s[warp][lane >> 2] = make_float2(m[0], l[0]);
-                ml_s[warp][(lane >> 2) + 8] = make_float2(m[1], l[1]);
-            }
-            __syncthreads();
-            float total[2], top[2];
+            const bool whole = first_chunk == 0 && row_done;
+            const int64_t part = 2 * int64_t(blockIdx.x) + (first_chunk == 0 ? 1 : 0);
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
-                const int row = (lane >> 2) + 8 * r;
-                float mm = -INFINITY;
+            for (int r = 0; r < HALVES; r++) {  // eight query heads at a time meet in shared memory
 #pragma unroll
-                for (int w = 0; w < kWarps; w++) mm = fmaxf(mm, ml_s[w][row].x);
-                const float rf = mm == -INFINITY ? 0.f : mm;
-                total[r] = 0.f;
+                for (int i = 0; i < NT; i++)
+                    *reinterpret_cast<float2*>(merge + Shape::merged(warp, lane >> 2, i * 8 + (lane & 3) * 2)) =
+                        make_float2(acc[i][2 * r], acc[i][2 * r + 1]);
+                __syncthreads();
+                const int d = (threadIdx.x % (DP / 2)) * 2;
+                for (int g = threadIdx.x / (DP / 2); g < 8; g += kThreads / (DP / 2)) {
+                    const int in_group = at.tile * 16 + 8 * r + g;
+                    if (in_group >= a.group || threadIdx.x >= kThreads / (DP / 2) * (DP / 2)) break;
+                    const Merged all(ml_s, 8 * r + g);
+                    float2 o = make_float2(0.f, 0.f);
 #pragma unroll
-                for (int w = 0; w < kWarps; w++) total[r] += ml_s[w][row].y * ex2(ml_s[w][row].x - rf);
-                top[r] = mm;
-                const float f = ex2(m[r] - rf);
-#pragma unroll
-                for (int i = 0; i < NT; i++) {
-                    acc[i][2 * r] *= f;
-                    acc[i][2 * r + 1] *= f;
-                }
-            }
-            float* slot = merge + (warp & 1) * (16 * DP) + lane;
-            if (warp >= 2) {
-#pragma unroll
-                for (int i = 0; i < NT * 4; i++) slot[i * 32] = acc[i >> 2][i & 3];
-            }
-            __syncthreads();
-            if (warp < 2) {
-#pragma unroll
-                for (int i = 0; i < NT * 4; i++) acc[i >> 2][i & 3] += slot[i * 32];
-                if (warp == 1) {
-#pragma unroll
-                    for (int i = 0; i < NT * 4; i++) slot[i * 32] = acc[i >> 2][i & 3];
-                }
-            }
-            __syncthreads();
-            if (warp == 0) {
-                const bool whole = first_chunk == 0 && at.chunk + 1 == at.chunks;
-                const int part = 2 * blockIdx.x + (first_chunk == 0 ? 1 : 0);
-                const float* other = merge + 16 * DP + lane;
-#pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    const int row = (lane >> 2) + 8 * r, in_group = at.tile * 16 + row;
-                    if (in_group >= a.group) continue;
+                    for (int w = 0; w < kWarps; w++) {
+                        const float2 x = *reinterpret_cast<const float2*>(merge + Shape::merged(w, g, d));
+                        o.x = fmaf(all.weight[w], x.x, o.x);
+                        o.y = fmaf(all.weight[w], x.y, o.y);
+                    }
                     const int64_t head = int64_t(at.kvh) * a.group + in_group;
                     if (whole) {
-                        const float inv = total[r] == 0.f ? 0.f : 1.f / total[r];
-                        T* o = O + at.b * a.os[0] + head * a.os[1];
-#pragma unroll
-                        for (int i = 0; i < NT; i++) {
-                            const int d = i * 8 + (lane & 3) * 2;
-                            if (d < a.D)
-                                *reinterpret_cast<uint32_t*>(o + d) = pack2<T>((acc[i][2 * r] + other[(i * 4 + 2 * r) * 32]) * inv,
-                                                                              (acc[i][2 * r + 1] + other[(i * 4 + 2 * r + 1) * 32]) * inv);
-                        }
-                        if (a.lse && (lane & 3) == 0)
-                            a.lse[at.b * int64_t(a.Hq) + head] = total[r] == 0.f ? -INFINITY : top[r] * kLn2 + logf(total[r]);
+                        const float inv = all.sum == 0.f ? 0.f : 1.f / all.sum;
+                        if (d < a.D) *reinterpret_cast<uint32_t*>(O + at.b * a.os[0] + head * a.os[1] + d) = pack2<T>(o.x * inv, o.y * inv);
+                        if (a.lse && d == 0) a.lse[at.b * int64_t(a.Hq) + head] = all.lse();
                     } else {
-                        float* o = a.part_o + (int64_t(part) * a.tile_rows + row) * a.D;
-#pragma unroll
-                        for (int i = 0; i < NT; i++) {
-                            const int d = i * 8 + (lane & 3) * 2;
-                            if (d < a.D)
-                                *reinterpret_cast<float2*>(o + d) = make_float2(acc[i][2 * r] + other[(i * 4 + 2 * r) * 32],
-                                                                                acc[i][2 * r + 1] + other[(i * 4 + 2 * r + 1) * 32]);
-                        }
-                        if ((lane & 3) == 0) a.part_ml[int64_t(part) * a.tile_rows + row] = make_float2(top[r], total[r]);
+                        if (d < a.D) *reinterpret_cast<float2*>(a.part_o + (part * a.tile_rows + 8 * r + g) * a.D + d) = o;
+                        if (d == 0) a.part_ml[part * a.tile_rows + 8 * r + g] = make_float2(all.top, all.sum);
                     }
                 }
-                if (u + 1 == units && lane == 0) {
-                    const bool begun = first_chunk == 0 && !whole;
-                    const int64_t row_end = run.end + (at.chunks - 1 - at.chunk);
-                    a.begun[blockIdx.x] = make_int4(begun ? row_of(a, at) : -1, int((row_end * run.blocks - 1) / run.total), 0, 0);
-                }
+                __syncthreads();  // the buffers are the next eight heads' or the next row's
             }
-            __syncthreads();
+            if (first_chunk == 0 && !whole) {
+                begun = row_of(a, at);
+                last = run.block_of(run.end + (at.chunks - 2 - at.chunk));
+            }
+            first_chunk = -1;
         }
-        at.next(a);
-    }
+        stage = stage + 1 == S ? 0 : stage + 1;
+    } while (at.next(a));
+    if (threadIdx.x == 0) a.begun[blockIdx.x] = make_int4(begun, last, 0, 0);
 }
 
 // ---- fp32, and whatever is not aligned for 16-byte copies: FMA units -------------------------------------------------------------
@@ -491,8 +515,7 @@ template <int DP, int GT> struct SimtShape {
     static constexpr int kPieces = DP / 4;                       // 16-byte pieces of a row
     static constexpr int kStage = 2 * kKeys * DP * 4;            // 8 KB
     static constexpr int kStages = 3;
-    static constexpr int kMerge = GT * DP * 4;
-    static constexpr int kBytes = kWarps * kStages * kStage + 2 * kMerge + GT * DP * 4;
+    static constexpr int kBytes = kWarps * kStages * kStage + (kWarps + 1) * GT * DP * 4;  // the ring, the warps' outputs, the queries
     static __device__ __forceinline__ int offset(int row, int piece) {  // in floats; eight lanes of a step read eight banks
         return row * DP + ((piece ^ ((row * kLanes) & 7)) << 2);
     }
@@ -511,7 +534,7 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const T* __restric
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     float* ring = reinterpret_cast<float*>(smem + warp * (S * Shape::kStage));
     float* merge = reinterpret_cast<float*>(smem + kWarps * S * Shape::kStage);
-    float* q_s = merge + 2 * GT * DP;
+    float* q_s = merge + kWarps * GT * DP;
     if (a.D < DP) {
         for (int i = lane; i < S * Shape::kStage / 4; i += 32) ring[i] = 0.f;
         __syncwarp();
@@ -524,8 +547,8 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const T* __restric
         if (threadIdx.x == 0) a.begun[blockIdx.x] = make_int4(-1, 0, 0, 0);
         return;
     }
-    const int units = int(run.end - run.begin);
     Cursor load = run.at, at = run.at;
+    bool more = true;  // the load cursor stands on a chunk that has not been asked for
     const int key_lane = warp * KS + (lane % KS);
     int key = load.lo + load.chunk * a.chunk + key_lane;
     int entry = page_entry(a, load, key);
@@ -566,27 +589,26 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const T* __restric
         if constexpr (ASYNC) cp_async_commit();
     };
     auto advance = [&]() {
-        load.next(a);
-        if (load.b < a.B) {
+        more = load.next(a);
+        if (more) {
             key = load.lo + load.chunk * a.chunk + key_lane;
             entry = page_entry(a, load, key);
         }
     };
-    int loaded = 0;
 #pragma unroll
     for (int s = 0; s < S - 1; s++) {
-        if (loaded < units) {
+        if (more) {
             issue(s);
-            if (++loaded < units) advance();
+            advance();
         } else if constexpr (ASYNC) {
             cp_async_commit();
         }
     }
 
     float acc[GT][C], m[GT], l[GT];
-    int first_chunk = 0;
-    for (int u = 0; u < units; u++) {
-        if (u == 0 || at.chunk == 0) {
+    int first_chunk = -1, begun = -1, last = 0, stage = 0;
+    do {
+        if (first_chunk < 0) {
             first_chunk = at.chunk;
             // the merge that ended the row before was followed by a barrier: nobody reads q_s any more
             for (int i = threadIdx.x; i < GT * DP; i += kThreads) {
@@ -606,13 +628,12 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const T* __restric
         }
         if constexpr (ASYNC) cp_async_wait<S - 2>();
         __syncwarp();
-        if (loaded < units) {
-            issue((u + S - 1) % S);
-            if (++loaded < units) advance();
+        if (more) {
+            issue(stage == 0 ? S - 1 : stage - 1);
+            advance();
         } else if constexpr (ASYNC) {
             cp_async_commit();
         }
-        const int stage = u % S;
         const uint32_t mask = mask_s[warp][stage];
         if (mask) {
             const float* kb = ring + stage * (Shape::kStage / 4);
@@ -677,77 +698,45 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const T* __restric
                 }
             }
         }
-        if (at.chunk + 1 == at.chunks || u + 1 == units) {
+        const bool row_done = at.chunk + 1 == at.chunks;
+        if (row_done || at.left == 1) {
+            float* mine = merge + warp * (GT * DP);
 #pragma unroll
             for (int g = 0; g < GT; g++) {
                 l[g] = warp_sum_f(l[g]);
                 if (lane == 0) ml_s[warp][g] = make_float2(m[g], l[g]);
+#pragma unroll
+                for (int c = 0; c < C; c++) mine[g * DP + (C == 2 ? lane * 2 + c : (c >> 2) * 128 + lane * 4 + (c & 3))] = acc[g][c];
             }
+            const bool whole = first_chunk == 0 && row_done;
+            const int64_t part = 2 * int64_t(blockIdx.x) + (first_chunk == 0 ? 1 : 0);
             __syncthreads();
-            float total[GT], top[GT];
+            for (int i = threadIdx.x; i < GT * DP; i += kThreads) {
+                const int g = i / DP, d = i % DP, in_group = at.tile * GT + g;
+                if (in_group >= a.group) break;
+                const Merged all(ml_s, g);
+                float o = 0.f;
 #pragma unroll
-            for (int g = 0; g < GT; g++) {
-                float mm = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < kWarps; w++) mm = fmaxf(mm, ml_s[w][g].x);
-                const float rf = mm == -INFINITY ? 0.f : mm;
-                total[g] = 0.f;
-#pragma unroll
-                for (int w = 0; w < kWarps; w++) total[g] += ml_s[w][g].y * ex2(ml_s[w][g].x - rf);
-                top[g] = mm;
-                const float f = ex2(m[g] - rf);
-#pragma unroll
-                for (int c = 0; c < C; c++) acc[g][c] *= f;
-            }
-            float* slot = merge + (warp & 1) * (GT * DP) + lane;
-            if (warp >= 2) {
-#pragma unroll
-                for (int i = 0; i < GT * C; i++) slot[i * 32] = acc[i / C][i % C];
-            }
-            __syncthreads();
-            if (warp < 2) {
-#pragma unroll
-                for (int i = 0; i < GT * C; i++) acc[i / C][i % C] += slot[i * 32];
-                if (warp == 1) {
-#pragma unroll
-                    for (int i = 0; i < GT * C; i++) slot[i * 32] = acc[i / C][i % C];
+                for (int w = 0; w < kWarps; w++) o = fmaf(all.weight[w], merge[w * (GT * DP) + i], o);
+                const int64_t head = int64_t(at.kvh) * a.group + in_group;
+                if (whole) {
+                    if (d < a.D) O[at.b * a.os[0] + head * a.os[1] + d] = from_float<T>(all.sum == 0.f ? 0.f : o / all.sum);
+                    if (a.lse && d == 0) a.lse[at.b * int64_t(a.Hq) + head] = all.lse();
+                } else {
+                    if (d < a.D) a.part_o[(part * a.tile_rows + g) * a.D + d] = o;
+                    if (d == 0) a.part_ml[part * a.tile_rows + g] = make_float2(all.top, all.sum);
                 }
             }
             __syncthreads();
-            if (warp == 0) {
-                const bool whole = first_chunk == 0 && at.chunk + 1 == at.chunks;
-                const int part = 2 * blockIdx.x + (first_chunk == 0 ? 1 : 0);
-                const float* other = merge + GT * DP + lane;
-#pragma unroll
-                for (int g = 0; g < GT; g++) {
-                    const int in_group = at.tile * GT + g;
-                    if (in_group >= a.group) continue;
-                    const int64_t head = int64_t(at.kvh) * a.group + in_group;
-                    const float inv = !whole ? 1.f : total[g] == 0.f ? 0.f : 1.f / total[g];
-#pragma unroll
-                    for (int c = 0; c < C; c++) {
-                        const int d = C == 2 ? lane * 2 + c : (c >> 2) * 128 + lane * 4 + (c & 3);
-                        if (d >= a.D) continue;
-                        const float o = (acc[g][c] + other[(g * C + c) * 32]) * inv;
-                        if (whole) O[at.b * a.os[0] + head * a.os[1] + d] = from_float<T>(o);
-                        else a.part_o[(int64_t(part) * a.tile_rows + g) * a.D + d] = o;
-                    }
-                    if (lane == 0) {
-                        if (!whole) a.part_ml[int64_t(part) * a.tile_rows + g] = make_float2(top[g], total[g]);
-                        else if (a.lse)
-                            a.lse[at.b * int64_t(a.Hq) + head] = total[g] == 0.f ? -INFINITY : top[g] * kLn2 + logf(total[g]);
-                    }
-                }
-                if (u + 1 == units && lane == 0) {
-                    const bool begun = first_chunk == 0 && !whole;
-                    const int64_t row_end = run.end + (at.chunks - 1 - at.chunk);
-                    a.begun[blockIdx.x] = make_int4(begun ? row_of(a, at) : -1, int((row_end * run.blocks - 1) / run.total), 0, 0);
-                }
+            if (first_chunk == 0 && !whole) {
+                begun = row_of(a, at);
+                last = run.block_of(run.end + (at.chunks - 2 - at.chunk));
             }
-            __syncthreads();
+            first_chunk = -1;
         }
-        at.next(a);
-    }
+        stage = stage + 1 == S ? 0 : stage + 1;
+    } while (at.next(a));
+    if (threadIdx.x == 0) a.begun[blockIdx.x] = make_int4(begun, last, 0, 0);
 }
 
 // ---- join ----------------------------------------------------------------------------------------------------------------------
@@ -841,18 +830,23 @@ int launch_join(Ctx* ctx, const PagedArgs& a, int blocks, T* O) {
     return after_launch(ctx, "paged_join_kernel");
 }
 
-template <typename T, int DP>
-int launch_tc(Ctx* ctx, PagedArgs& a, int blocks, const T* Q, const T* K, const T* V, T* O) {
+template <typename T, int DP, int HALVES>
+int launch_tc_rows(Ctx* ctx, PagedArgs& a, int blocks, const T* Q, const T* K, const T* V, T* O) {
     a.tile_rows = kTcRows;
     a.tiles = int(ceil_div(a.group, kTcRows));
     if (a.tiles == 1) a.tile_rows = a.group;  // the scratch holds no rows that do not exist
     a.chunk = kWarps * 16;
-    auto kernel = paged_tc_kernel<T, DP>;
+    auto kernel = paged_tc_kernel<T, DP, HALVES>;
     static std::atomic<unsigned> done{0};
     DOCC_TRY(set_smem(ctx, done, kernel, TcShape<DP>::kBytes));
     DOCC_CUDA_TRY(launch_pdl(kernel, dim3(unsigned(blocks)), dim3(kThreads), TcShape<DP>::kBytes, ctx->stream, Q, K, V, O, a));
     DOCC_TRY(after_launch(ctx, "paged_tc_kernel"));
     return launch_join<T>(ctx, a, blocks, O);
+}
+
+template <typename T, int DP>
+int launch_tc(Ctx* ctx, PagedArgs& a, int blocks, const T* Q, const T* K, const T* V, T* O) {
+    return a.group <= 8 ? launch_tc_rows<T, DP, 1>(ctx, a, blocks, Q, K, V, O) : launch_tc_rows<T, DP, 2>(ctx, a, blocks, Q, K, V, O);
 }
 
 template <typename T, int DP, int GT, bool ASYNC>
