@@ -43,11 +43,13 @@ struct PagedArgs {
     const int32_t* lengths;
     float* lse;
     DeviceStatus* status;
-    // scratch: two partial results per block (the row it finished for an earlier block, the row it began), and per block the
-    // row it began and did not finish
-    float* part_o;    // [2 * blocks][tile_rows][D]
+    // scratch: two partial results per block (the row it finished for an earlier block, the row it began), and which rows are in
+    // parts: an entry per row where there are fewer rows than blocks, else one per block for the row it began and did not finish
+    int part_d;       // D rounded up to a multiple of 4
+    float* part_o;    // [2 * blocks][tile_rows][part_d]
     float2* part_ml;  // [2 * blocks][tile_rows]: maximum (of s log2 e), sum
-    int4* begun;      // [blocks]: {row or -1, last block of the row, 0, 0}
+    int4* split;      // {row or -1, its first block, its last block, 0}
+    int by_row;
 };
 
 // Visible tokens [lo, n) of sequence b.
@@ -266,7 +268,7 @@ template <int DP> struct TcShape {
 
 // HALVES: 1 where the tile has at most eight query heads (rows 8-15 of the fragments are padding), else 2.
 template <typename T, int DP, int HALVES>
-__global__ void __launch_bounds__(kThreads) paged_tc_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
+__global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) paged_tc_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
                                                             T* __restrict__ O, PagedArgs a) {
     using Shape = TcShape<DP>;
     constexpr int S = Shape::kStages, PIECES = DP / 8, NT = DP / 8;
@@ -287,7 +289,7 @@ __global__ void __launch_bounds__(kThreads) paged_tc_kernel(const T* __restrict_
 
     Run run;
     if (!find_run(a, run)) {
-        if (threadIdx.x == 0) a.begun[blockIdx.x] = make_int4(-1, 0, 0, 0);
+        if (threadIdx.x == 0 && !a.by_row) a.split[blockIdx.x] = make_int4(-1, 0, 0, 0);
         return;
     }
     Cursor load = run.at, at = run.at;
@@ -489,21 +491,24 @@ __global__ void __launch_bounds__(kThreads) paged_tc_kernel(const T* __restrict_
                         if (d < a.D) *reinterpret_cast<uint32_t*>(O + at.b * a.os[0] + head * a.os[1] + d) = pack2<T>(o.x * inv, o.y * inv);
                         if (a.lse && d == 0) a.lse[at.b * int64_t(a.Hq) + head] = all.lse();
                     } else {
-                        if (d < a.D) *reinterpret_cast<float2*>(a.part_o + (part * a.tile_rows + 8 * r + g) * a.D + d) = o;
+                        if (d < a.D) *reinterpret_cast<float2*>(a.part_o + (part * a.tile_rows + 8 * r + g) * a.part_d + d) = o;
                         if (d == 0) a.part_ml[part * a.tile_rows + 8 * r + g] = make_float2(all.top, all.sum);
                     }
                 }
                 __syncthreads();  // the buffers are the next eight heads' or the next row's
             }
-            if (first_chunk == 0 && !whole) {
-                begun = row_of(a, at);
-                last = run.block_of(run.end + (at.chunks - 2 - at.chunk));
+            if (first_chunk == 0) {
+                if (!whole) {
+                    begun = row_of(a, at);
+                    last = run.block_of(run.end + (at.chunks - 2 - at.chunk));
+                }
+                if (a.by_row && threadIdx.x == 0) a.split[row_of(a, at)] = make_int4(begun, blockIdx.x, last, 0);
             }
             first_chunk = -1;
         }
         stage = stage + 1 == S ? 0 : stage + 1;
     } while (at.next(a));
-    if (threadIdx.x == 0) a.begun[blockIdx.x] = make_int4(begun, last, 0, 0);
+    if (threadIdx.x == 0 && !a.by_row) a.split[blockIdx.x] = make_int4(begun, blockIdx.x, last, 0);
 }
 
 // ---- fp32, and whatever is not aligned for 16-byte copies: FMA units -------------------------------------------------------------
@@ -522,7 +527,7 @@ template <int DP, int GT> struct SimtShape {
 };
 
 template <typename T, int DP, int GT, bool ASYNC>
-__global__ void __launch_bounds__(kThreads) paged_simt_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
+__global__ void __launch_bounds__(kThreads, 2) paged_simt_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
                                                               T* __restrict__ O, PagedArgs a) {
     using Shape = SimtShape<DP, GT>;
     constexpr int S = Shape::kStages, KS = Shape::kKeys, LPK = Shape::kLanes, PIECES = Shape::kPieces, C = DP / 32;
@@ -544,7 +549,7 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const T* __restric
 
     Run run;
     if (!find_run(a, run)) {
-        if (threadIdx.x == 0) a.begun[blockIdx.x] = make_int4(-1, 0, 0, 0);
+        if (threadIdx.x == 0 && !a.by_row) a.split[blockIdx.x] = make_int4(-1, 0, 0, 0);
         return;
     }
     Cursor load = run.at, at = run.at;
@@ -723,75 +728,80 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const T* __restric
                     if (d < a.D) O[at.b * a.os[0] + head * a.os[1] + d] = from_float<T>(all.sum == 0.f ? 0.f : o / all.sum);
                     if (a.lse && d == 0) a.lse[at.b * int64_t(a.Hq) + head] = all.lse();
                 } else {
-                    if (d < a.D) a.part_o[(part * a.tile_rows + g) * a.D + d] = o;
+                    if (d < a.D) a.part_o[(part * a.tile_rows + g) * a.part_d + d] = o;
                     if (d == 0) a.part_ml[part * a.tile_rows + g] = make_float2(all.top, all.sum);
                 }
             }
             __syncthreads();
-            if (first_chunk == 0 && !whole) {
-                begun = row_of(a, at);
-                last = run.block_of(run.end + (at.chunks - 2 - at.chunk));
+            if (first_chunk == 0) {
+                if (!whole) {
+                    begun = row_of(a, at);
+                    last = run.block_of(run.end + (at.chunks - 2 - at.chunk));
+                }
+                if (a.by_row && threadIdx.x == 0) a.split[row_of(a, at)] = make_int4(begun, blockIdx.x, last, 0);
             }
             first_chunk = -1;
         }
         stage = stage + 1 == S ? 0 : stage + 1;
     } while (at.next(a));
-    if (threadIdx.x == 0) a.begun[blockIdx.x] = make_int4(begun, last, 0, 0);
+    if (threadIdx.x == 0 && !a.by_row) a.split[blockIdx.x] = make_int4(begun, blockIdx.x, last, 0);
 }
 
 // ---- join ----------------------------------------------------------------------------------------------------------------------
-// Block (c, r): query head r of the row that block c of the first kernel began and did not finish; its parts lie in the blocks up to
-// `last`, the first as the row begun, the others as the row finished for an earlier block. Four groups of threads take every fourth
-// part.
-constexpr int kJoinGroups = 4;
-template <typename T, int DP>
-__global__ void __launch_bounds__(kJoinGroups * DP) paged_join_kernel(T* __restrict__ O, PagedArgs a) {
-    extern __shared__ float weight_s[];  // one per part
-    __shared__ float red[kJoinGroups][DP];
-    __shared__ float total_s;
+// Block (x, y, z): entry x of `split`, query head y of its tile, columns [z width, (z + 1) width). The row's parts lie in blocks first ..
+// last: the first as the row begun, the others as the row finished for an earlier block. A part's columns are width / 4 lanes' (four
+// each), the rest of the block's threads take other parts. The code is kept small: the kernel runs for a few microseconds, and
+// unrolled eight-fold its instructions took longer to arrive than its data (17 against 11 against 7.4 us for 148 parts, caches cold).
+constexpr int kJoinThreads = 256;
+
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(T* __restrict__ O, PagedArgs a, int width) {
+    __shared__ float4 sum_s[kJoinThreads / 32][32];
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
-    const int4 begun = a.begun[blockIdx.x];
-    if (begun.x < 0) return;
-    const int r = blockIdx.y, tile = begun.x % a.tiles, in_group = tile * a.tile_rows + r;
-    if (in_group >= a.group) return;
-    const int kvh = begun.x / a.tiles % a.Hkv, b = begun.x / a.tiles / a.Hkv;
-    const int parts = begun.y - int(blockIdx.x) + 1;
-    auto part = [&](int i) { return int64_t(2 * (int(blockIdx.x) + i) + (i == 0 ? 1 : 0)) * a.tile_rows + r; };
-    if (threadIdx.x < 32) {
-        float top = -INFINITY, sum = 0.f;
-        for (int i = threadIdx.x; i < parts; i += 32) top = fmaxf(top, a.part_ml[part(i)].x);
-        top = warp_max_f(top);
-        const float ref = top == -INFINITY ? 0.f : top;
-        for (int i = threadIdx.x; i < parts; i += 32) {
-            const float2 ml = a.part_ml[part(i)];
-            const float w = ex2(ml.x - ref);
-            weight_s[i] = w;
-            sum += w * ml.y;
-        }
-        sum = warp_sum_f(sum);
-        if (threadIdx.x == 0) {
-            total_s = sum;
-            if (a.lse) a.lse[b * int64_t(a.Hq) + int64_t(kvh) * a.group + in_group] = sum == 0.f ? -INFINITY : top * kLn2 + logf(sum);
-        }
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = int(blockIdx.y);
+    const int4 entry = a.split[blockIdx.x];
+    if (entry.x < 0) return;
+    const int first = entry.y, parts = entry.z - first + 1;
+    const int tile = entry.x % a.tiles, kvh = entry.x / a.tiles % a.Hkv, b = entry.x / a.tiles / a.Hkv;
+    if (tile * a.tile_rows + r >= a.group) return;
+    auto part = [&](int i) { return (2 * (first + i) + (i == 0 ? 1 : 0)) * a.tile_rows + r; };
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll 2
+    for (int i = lane; i < parts; i += 32) {
+        const float2 ml = a.part_ml[part(i)];
+        const float next = fmaxf(top, ml.x), ref = next == -INFINITY ? 0.f : next;
+        sum = sum * ex2(top - ref) + ml.y * ex2(ml.x - ref);
+        top = next;
     }
+    const float all = warp_max_f(top), ref = all == -INFINITY ? 0.f : all;
+    sum = warp_sum_f(sum * ex2(top - ref));
+
+    const int lanes = width / 4;  // to a part: 8, 16 or 32
+    const int d = int(blockIdx.z) * width + (lane & (lanes - 1)) * 4;
+    const float* columns = a.part_o + (d < a.part_d ? d : 0);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+    for (int i = int(threadIdx.x) / lanes; i < parts; i += int(blockDim.x) / lanes) {
+        const float4 x = *reinterpret_cast<const float4*>(columns + int64_t(part(i)) * a.part_d);
+        const float f = ex2(a.part_ml[part(i)].x - ref);
+        o.x = fmaf(f, x.x, o.x); o.y = fmaf(f, x.y, o.y); o.z = fmaf(f, x.z, o.z); o.w = fmaf(f, x.w, o.w);
+    }
+#pragma unroll 1
+    for (int s = lanes; s < 32; s <<= 1) {
+        o.x += __shfl_xor_sync(0xffffffffu, o.x, s); o.y += __shfl_xor_sync(0xffffffffu, o.y, s);
+        o.z += __shfl_xor_sync(0xffffffffu, o.z, s); o.w += __shfl_xor_sync(0xffffffffu, o.w, s);
+    }
+    if (lane < lanes) sum_s[warp][lane] = o;
     __syncthreads();
-    const int d = threadIdx.x % DP, group = threadIdx.x / DP;
-    float o = 0.f;
-    if (d < a.D) {
-#pragma unroll 8
-        for (int i = group; i < parts; i += kJoinGroups) {
-            const float w = weight_s[i];
-            if (w != 0.f) o = fmaf(w, a.part_o[part(i) * a.D + d], o);
-        }
+    const int64_t head = int64_t(kvh) * a.group + tile * a.tile_rows + r;
+    const int column = int(blockIdx.z) * width + int(threadIdx.x);
+    if (int(threadIdx.x) < width && column < a.D) {
+        float v = 0.f;
+        for (int w = 0; w < int(blockDim.x >> 5); w++) v += reinterpret_cast<const float*>(sum_s[w])[threadIdx.x];
+        O[b * a.os[0] + head * a.os[1] + column] = from_float<T>(sum == 0.f ? 0.f : v / sum);
     }
-    red[group][d] = o;
-    __syncthreads();
-    if (group == 0 && d < a.D) {
-#pragma unroll
-        for (int g = 1; g < kJoinGroups; g++) o += red[g][d];
-        O[b * a.os[0] + (int64_t(kvh) * a.group + in_group) * a.os[1] + d] = from_float<T>(total_s == 0.f ? 0.f : o / total_s);
-    }
+    if (a.lse && column == 0) a.lse[b * int64_t(a.Hq) + head] = sum == 0.f ? -INFINITY : all * kLn2 + logf(sum);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------
@@ -806,7 +816,7 @@ Scratch scratch_of(int blocks, int64_t group, int64_t D) {
     Scratch s;
     s.ml_at = (size_t(blocks) * sizeof(int4) + 255) / 256 * 256;
     s.o_at = s.ml_at + (parts * rows * sizeof(float2) + 255) / 256 * 256;
-    s.bytes = s.o_at + parts * rows * size_t(D) * 4;
+    s.bytes = s.o_at + parts * rows * size_t(ceil_div(D, 4) * 4) * 4;
     return s;
 }
 int blocks_of(Ctx* ctx, int64_t D) { return ctx->sm_count * (D <= 128 ? 2 : 1); }
@@ -822,11 +832,16 @@ template <typename F> int set_smem(Ctx* ctx, std::atomic<unsigned>& done, F kern
 
 template <typename T>
 int launch_join(Ctx* ctx, const PagedArgs& a, int blocks, T* O) {
-    const dim3 grid(unsigned(blocks), unsigned(a.group < a.tile_rows ? a.group : a.tile_rows));
-    const size_t smem = size_t(blocks) * 4;
-    if (a.D <= 64) DOCC_CUDA_TRY(launch_pdl(paged_join_kernel<T, 64>, grid, dim3(kJoinGroups * 64), smem, ctx->stream, O, a));
-    else if (a.D <= 128) DOCC_CUDA_TRY(launch_pdl(paged_join_kernel<T, 128>, grid, dim3(kJoinGroups * 128), smem, ctx->stream, O, a));
-    else DOCC_CUDA_TRY(launch_pdl(paged_join_kernel<T, 256>, grid, dim3(kJoinGroups * 256), smem, ctx->stream, O, a));
+    const int entries = a.by_row ? int(int64_t(a.B) * a.Hkv * a.tiles) : blocks, heads = a.group < a.tile_rows ? a.group : a.tile_rows;
+    // The fewer rows there are, the more parts each is in: 256 threads and narrow columns, hence up to 32 parts at a time, as long as
+    // all blocks still run together; with many entries, most of which are gone after one load, 128 threads and whole rows.
+    int width = 128, threads = 128;
+    if (int64_t(entries) * heads <= int64_t(ctx->sm_count) * 4) {
+        threads = kJoinThreads;
+        while (width > 32 && int64_t(entries) * heads * ceil_div(a.D, width / 2) <= int64_t(ctx->sm_count) * 4) width /= 2;
+    }
+    const dim3 grid(unsigned(entries), unsigned(heads), unsigned(ceil_div(a.D, width)));
+    DOCC_CUDA_TRY(launch_pdl(paged_join_kernel<T>, grid, dim3(unsigned(threads)), 0, ctx->stream, O, a, width));
     return after_launch(ctx, "paged_join_kernel");
 }
 
@@ -836,6 +851,7 @@ int launch_tc_rows(Ctx* ctx, PagedArgs& a, int blocks, const T* Q, const T* K, c
     a.tiles = int(ceil_div(a.group, kTcRows));
     if (a.tiles == 1) a.tile_rows = a.group;  // the scratch holds no rows that do not exist
     a.chunk = kWarps * 16;
+    a.by_row = int64_t(a.B) * a.Hkv * a.tiles <= blocks;
     auto kernel = paged_tc_kernel<T, DP, HALVES>;
     static std::atomic<unsigned> done{0};
     DOCC_TRY(set_smem(ctx, done, kernel, TcShape<DP>::kBytes));
@@ -855,6 +871,7 @@ int launch_simt(Ctx* ctx, PagedArgs& a, int blocks, const T* Q, const T* K, cons
     a.tiles = int(ceil_div(a.group, GT));
     if (a.tiles == 1) a.tile_rows = a.group;
     a.chunk = kWarps * SimtShape<DP, GT>::kKeys;
+    a.by_row = int64_t(a.B) * a.Hkv * a.tiles <= blocks;
     auto kernel = paged_simt_kernel<T, DP, GT, ASYNC>;
     static std::atomic<unsigned> done{0};
     DOCC_TRY(set_smem(ctx, done, kernel, SimtShape<DP, GT>::kBytes));
@@ -943,6 +960,9 @@ extern "C" int docc_b200_paged_attention(int prec, int64_t B, int64_t Hq, int64_
         DOCC_REQUIRE(workspace_bytes >= scratch.bytes && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
                      "paged_attention: the workspace needs %zu bytes on a 16-byte boundary", scratch.bytes);
     } else {
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        DOCC_CUDA_TRY(cudaStreamIsCapturing(ctx->stream, &capture));
+        DOCC_REQUIRE(capture == cudaStreamCaptureStatusNone, "paged_attention: a captured call needs a workspace of its own");
         DOCC_TRY(get_workspace(ctx, 3, scratch.bytes, &workspace));
     }
     PagedArgs a;
@@ -957,7 +977,8 @@ extern "C" int docc_b200_paged_attention(int prec, int64_t B, int64_t Hq, int64_
     }
     a.num_pages = num_pages; a.page_size = uint32_t(page_size); a.max_pages = max_pages; a.table_stride = table_stride;
     a.page_table = page_table; a.lengths = lengths; a.lse = static_cast<float*>(lse); a.status = ctx->status_dev;
-    a.begun = static_cast<int4*>(workspace);
+    a.part_d = int(ceil_div(D, 4) * 4);
+    a.split = static_cast<int4*>(workspace);
     a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + scratch.ml_at);
     a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + scratch.o_at);
     if (!Kcache) Kcache = Q;  // an empty cache: nothing of it is read, but copies of no bytes want an address

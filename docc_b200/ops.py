@@ -615,6 +615,12 @@ def rope_append(q, k, v, positions, inv_freq, k_cache, v_cache, slots, interleav
     return out
 
 
+def _capturing():
+    import torch
+
+    return torch.cuda.is_current_stream_capturing()
+
+
 _scratch_bytes = {}  # (device, query heads per key-value head, D) -> bytes: what the size of the scratch depends on
 
 
@@ -625,7 +631,8 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, scale=None, softca
     the scores (``docc_b200_paged_attention``). Returns the output [B, Hq, D], with ``return_lse`` also the float32 [B, Hq]
     logarithm of the softmax's denominator. Sequences of length 0 give zeros and -inf. Device tensors only.
 
-    With torch tensors the scratch comes from torch's allocator, so a captured graph owns the scratch it replays with."""
+    While torch captures a graph the scratch comes from torch's allocator, so that the graph owns what it replays with; otherwise it
+    is the library's, ordered on the calling thread's stream."""
     if _side(q, k_cache, v_cache, page_table, lengths, out):
         raise TypeError("paged_attention: the cache lives on the device; host arrays are not taken")
     if q.ndim != 3 or k_cache.ndim != 4:
@@ -643,7 +650,7 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, scale=None, softca
     out = _out_like(q, out, "paged_attention")
     lse = _new(q, (B, Hq), "float32") if return_lse else None
     work, bytes_ = None, 0
-    if _is_torch(q):
+    if _is_torch(q) and _capturing():
         key = (q.get_device(), Hq // Hkv, D)
         bytes_ = _scratch_bytes.get(key)
         if bytes_ is None:

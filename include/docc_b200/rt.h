@@ -306,9 +306,9 @@ int docc_b200_rope_append(int prec, int64_t tokens, int64_t Hq, int64_t Hkv, int
  * left out; both are reported by docc_b200_sync as DOCC_B200_ERR_BAD_INDEX.
  * Strides: Q, O [sb,sh]; caches [sp,sh,ss] as above; NULL = contiguous. D <= 256, prec 's', 'b', 'h'.
  * The scratch holds partial results of sequences that several blocks share. workspace == NULL uses
- * the calling thread's own (ordered on its stream); a caller that captures graphs which may run at
- * the same time passes one per graph, of docc_b200_paged_attention_workspace() bytes. Device
- * pointers only. */
+ * the calling thread's own (ordered on its stream); a captured call has to bring its own, of
+ * docc_b200_paged_attention_workspace() bytes, so that graphs which run at the same time do not
+ * share one. Device pointers only. */
 int docc_b200_paged_attention(int prec, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, float scale, float softcap, int64_t window,
                               const void* Q, const int64_t* q_strides /*[sb,sh] or NULL*/,
                               const void* Kcache, const int64_t* kc_strides, const void* Vcache, const int64_t* vc_strides,
