@@ -6,12 +6,12 @@
 // Bound by reading the logits once. Sums are kept per thread in units of log 2 against a reference r that need not be the maximum:
 // it is raised when a value lies 16 above it, so that in practice nothing is rescaled after a thread's first values.
 //
-// The alternatives cost no second pass. A thread keeps its largest logit and where it stood; the k-th largest of the threads' maxima
-// is a lower bound T of the row's k-th largest, and only threads whose maximum reaches T can hold others: about k of 256. Their
-// logits, k / 256 of the row, are read again (from L2), and what reaches T, few more than k values, is sorted.
+// The alternatives cost no second pass. A thread keeps its largest logit; T, a value that at least k threads' maxima reach, is a lower
+// bound of the row's k-th largest, and only those threads can hold others: some thirty of 256 for k = 20. Their logits are read again
+// (from L2), and what reaches T, few more than k values, is ranked by counting.
 //
-// With fewer rows than fill the machine, a cluster of up to eight blocks takes a row; their sums and sorted lists meet in the first
-// block's registers through distributed shared memory, in the order of the ranks.
+// With fewer rows than fill the machine, a cluster of up to eight blocks takes a row; the other blocks' sums and lists meet in the first
+// block through distributed shared memory, in the order of the ranks.
 #include "common.cuh"
 #include "device_math.cuh"
 #include "ptx.cuh"
@@ -110,41 +110,6 @@ template <typename T> __device__ __noinline__ void row_carefully(const T* x, con
     }
 }
 
-// ---- sorting keys, one per lane, in descending order --------------------------------------------------------------------------
-__device__ __forceinline__ uint64_t exchange(uint64_t v, int stride, bool larger) {
-    const uint64_t o = __shfl_xor_sync(0xffffffffu, v, stride);
-    return (v > o) == larger ? v : o;
-}
-__device__ __forceinline__ uint64_t sort32(uint64_t v, int lane) {
-#pragma unroll
-    for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-        for (int stride = size >> 1; stride > 0; stride >>= 1) v = exchange(v, stride, ((lane & stride) == 0) == ((lane & size) == 0));
-    return v;
-}
-// the 32 largest of two sorted lists
-__device__ __forceinline__ uint64_t merge32(uint64_t a, uint64_t b, int lane) {
-    const uint64_t r = __shfl_sync(0xffffffffu, b, 31 - lane);
-    uint64_t v = a > r ? a : r;
-#pragma unroll
-    for (int stride = 16; stride > 0; stride >>= 1) v = exchange(v, stride, (lane & stride) == 0);
-    return v;
-}
-// Every warp holds a sorted list; list[0] receives the 32 largest of all of them. Ends with a barrier.
-__device__ __forceinline__ uint64_t tournament(uint64_t mine, uint64_t (*list)[32], int lane, int warp) {
-    list[warp][lane] = mine;
-    __syncthreads();
-#pragma unroll
-    for (int half = kLpWarps / 2; half > 0; half >>= 1) {
-        if (warp < half) {
-            mine = merge32(mine, list[warp + half][lane], lane);
-            list[warp][lane] = mine;
-        }
-        __syncthreads();
-    }
-    return list[0][lane];
-}
-
 // ---- the one pass ----------------------------------------------------------------------------------------------------------------
 struct Sums {
     float ref, s0, s1;  // reference and sums in units of log 2
@@ -173,55 +138,169 @@ __device__ __forceinline__ Sums warp_join(Sums v) {
 
 constexpr float kHeadroom = 16.f;
 
-template <bool TOP> struct Scan {
-    float c;               // scale log2 e
-    float ref, limit;      // limit: the logit whose multiple by c lies kHeadroom above ref
-    float s0, s1;
-    float best;            // largest logit so far, and the first of the values it was found among
-    int best_at;
-    __device__ __forceinline__ explicit Scan(float c_) : c(c_), ref(0.f), limit(-INFINITY), s0(0.f), s1(0.f), best(-INFINITY), best_at(0) {}
-    template <int N> __device__ __forceinline__ void take(const float (&x)[N], int at) {
-        float top = x[0];
+// A 16-byte pack: its largest value, and its values raised to at least floor() so that no multiple of them is infinite and nothing
+// times 0 becomes a NaN. 16-bit packs do both on pairs. A NaN is passed over by the first and kept by the second.
+template <typename T> struct Packed;
+template <> struct Packed<float> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ float floor() { return -1e30f; }
+    static __device__ __forceinline__ float top(const uint4& w) {
+        return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
+    }
+    static __device__ __forceinline__ void values(const uint4& w, float (&x)[4]) {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int e = 1; e < N; e++) top = fmaxf(top, x[e]);
-        if (top > limit) {
-            // -inf, or a product beyond fp32: such values are left at 0 until a usable one comes (if none does, the row is taken carefully)
-            const float r = top * c;
-            const float next = r == -INFINITY ? 0.f : r;
-            if (s0 != 0.f) {
-                const float d = fmaxf(ref - next, -200.f), f = lp_ex2(d);
-                s1 = fmaf(s0, d, s1) * f;
-                s0 *= f;
-            }
-            ref = next;
-            limit = r == -INFINITY ? -INFINITY : top + kHeadroom / c;
-        }
-        if (TOP && top > best) {
-            best = top;
-            best_at = at;
-        }
+        for (int i = 0; i < 4; i++) x[i] = lp_max_nan(__uint_as_float(u[i]), floor());
+    }
+};
+template <> struct Packed<__nv_bfloat16> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ float floor() { return __uint_as_float(0xf1490000u); }  // -1e30
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ float top(const uint4& w) {
+        const uint32_t m = max2(max2(w.x, w.y), max2(w.z, w.w));
+        return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+    }
+    static __device__ __forceinline__ void values(const uint4& w, float (&x)[8]) {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int e = 0; e < N; e++) {
-            const float d = lp_max_nan(fmaf(x[e], c, -ref), -200.f);  // finite, so that nothing times 0 is NaN; a NaN stays
-            const float p = lp_ex2(d);
-            s0 += p;
-            s1 = fmaf(d, p, s1);
+        for (int i = 0; i < 4; i++) {
+            uint32_t r;
+            asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(u[i]), "r"(0xf149f149u));
+            x[2 * i] = __uint_as_float(r << 16);
+            x[2 * i + 1] = __uint_as_float(r & 0xffff0000u);
+        }
+    }
+};
+template <> struct Packed<__half> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ float floor() { return -65504.f; }
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ float top(const uint4& w) {
+        const uint32_t m = max2(max2(w.x, w.y), max2(w.z, w.w));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&m));
+        return fmaxf(f.x, f.y);
+    }
+    static __device__ __forceinline__ void values(const uint4& w, float (&x)[8]) {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            uint32_t r;
+            asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(u[i]), "r"(0xfbfffbffu));
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r));
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
         }
     }
 };
 
+struct Scan {
+    float c;           // scale log2 e
+    float ref, limit;  // limit: the logit whose multiple by c lies kHeadroom above ref
+    float best;        // largest logit so far
+    float2 s0, s1;     // sums of the even and the odd values
+    __device__ __forceinline__ explicit Scan(float c_)
+        : c(c_), ref(0.f), limit(-INFINITY), best(-INFINITY), s0(make_float2(0.f, 0.f)), s1(make_float2(0.f, 0.f)) {}
+    __device__ __forceinline__ void rise(float top) {
+        if (top > limit) {
+            // -inf, or a product beyond fp32: such values count nothing until a usable one comes (if none does, the row is taken carefully)
+            const float r = top * c;
+            const float next = r == -INFINITY ? 0.f : r;
+            const float d = fmaxf(ref - next, -200.f), f = lp_ex2(d);
+            if (s0.x + s0.y != 0.f) {
+                s1 = make_float2(fmaf(s0.x, d, s1.x) * f, fmaf(s0.y, d, s1.y) * f);
+                s0 = make_float2(s0.x * f, s0.y * f);
+            }
+            ref = next;
+            limit = r == -INFINITY ? -INFINITY : top + kHeadroom / c;
+        }
+        best = fmaxf(best, top);
+    }
+    __device__ __forceinline__ void one(float v, float floor) {
+        rise(v);
+        const float d = fmaf(lp_max_nan(v, floor), c, -ref), p = lp_ex2(d);
+        s0.x += p;
+        s1.x = fmaf(d, p, s1.x);
+    }
+    template <typename T> __device__ __forceinline__ void pack(const uint4& w) {
+        rise(Packed<T>::top(w));
+        float x[Packed<T>::N];
+        Packed<T>::values(w, x);
+#pragma unroll
+        for (int e = 0; e < Packed<T>::N; e += 2) {  // packed pairs: one instruction for two products or sums
+            float d0, d1;
+            asm("{\n.reg .b64 a, b, k, r;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %4};\nmov.b64 k, {%5, %5};\nfma.rn.f32x2 r, a, b, k;\n"
+                "mov.b64 {%0, %1}, r;\n}"
+                : "=f"(d0), "=f"(d1)
+                : "f"(x[e]), "f"(x[e + 1]), "f"(c), "f"(-ref));
+            const float p0 = lp_ex2(d0), p1 = lp_ex2(d1);
+            asm("{\n.reg .b64 a, b, r;\nmov.b64 a, {%0, %1};\nmov.b64 b, {%2, %3};\nadd.rn.f32x2 r, a, b;\nmov.b64 {%0, %1}, r;\n}"
+                : "+f"(s0.x), "+f"(s0.y)
+                : "f"(p0), "f"(p1));
+            asm("{\n.reg .b64 a, b, k, r;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 k, {%0, %1};\nfma.rn.f32x2 r, a, b, k;\n"
+                "mov.b64 {%0, %1}, r;\n}"
+                : "+f"(s1.x), "+f"(s1.y)
+                : "f"(d0), "f"(d1), "f"(p0), "f"(p1));
+        }
+    }
+    __device__ __forceinline__ Sums sums() const { return Sums{ref, s0.x + s0.y, s1.x + s1.y}; }
+};
+
+__device__ __forceinline__ uint32_t ordered(float x) { return uint32_t(rank_key(x, 0) >> 32); }
+
+// A value (as ordered bits) that at least k of the block's threads reach with theirs, near the k-th largest: a warp's j-th largest,
+// j = ceil(k / warps), of the r-th best warp, j r >= k. `values_s` has room for one word per warp. 0 if there is none.
+__device__ __forceinline__ uint32_t bound_of(uint32_t mine, int k, uint32_t* values_s, int lane, int warp) {
+    const int j = (k + kLpWarps - 1) / kLpWarps, r = (k + j - 1) / j;
+    uint32_t rest = mine, nth = 0;
+    for (int i = 0; i < j; i++) {
+        nth = __reduce_max_sync(0xffffffffu, rest);
+        if (lane == __ffs(__ballot_sync(0xffffffffu, rest == nth)) - 1) rest = 0;
+    }
+    if (lane == 0) values_s[warp] = nth;
+    __syncthreads();
+    const uint32_t v = lane < kLpWarps ? values_s[lane] : 0;
+    int above = 0;
+#pragma unroll
+    for (int w = 0; w < kLpWarps; w++) {
+        const uint32_t o = __shfl_sync(0xffffffffu, v, w);
+        above += o > v || (o == v && w < lane);
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, lane < kLpWarps && above == r - 1);
+    return __shfl_sync(0xffffffffu, v, __ffs(hit) - 1);
+}
+// The k largest of n distinct keys, in order: a key's place is the number of keys above it. Places past the last key hold 0.
+__device__ __forceinline__ void rank_keys(const uint64_t* keys, int n, int k, uint64_t* out) {
+    if (int(threadIdx.x) < k && int(threadIdx.x) >= n) out[threadIdx.x] = 0;
+    for (int i = threadIdx.x; i < n; i += kBlock) {
+        const uint64_t mine = keys[i];
+        int above = 0;
+#pragma unroll 4
+        for (int j = 0; j < n; j++) above += keys[j] > mine;
+        if (above < k && mine != 0) out[above] = mine;
+    }
+}
+
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kBlock) logprobs_kernel(const T* __restrict__ X, LogpArgs a, int ranks) {
     constexpr int VEC = 16 / sizeof(T), UNROLL = 4;
-    using P = Pack<T, VEC>;
     __shared__ Sums sums_s[kLpWarps];
     __shared__ float red_s[kLpWarps];
+    __shared__ uint32_t values_s[kLpWarps];
     __shared__ unsigned long long best_s;
-    __shared__ uint64_t list_s[kLpWarps][32];
+    __shared__ uint64_t list_s[kMaxTop];
     __shared__ uint64_t found_s[TOP ? kCandidates : 1];
     __shared__ int streams_s[TOP ? kBlock : 1];
     __shared__ int n_streams, n_found;
-    __shared__ Sums block_s;  // read by the cluster's first block
+    __shared__ Sums block_s;  // read, like list_s, by the cluster's first block
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -235,48 +314,29 @@ __global__ void __launch_bounds__(kBlock) logprobs_kernel(const T* __restrict__ 
         if (head > vocab) head = vocab;
         const int packs = (vocab - head) / VEC, tail0 = head + packs * VEC;
         const int p0 = int(int64_t(packs) * rank / ranks), p1 = int(int64_t(packs) * (rank + 1) / ranks);
-        const P* xp = reinterpret_cast<const P*>(x + head);
+        const uint4* xp = reinterpret_cast<const uint4*>(x + head);
 
-        Scan<TOP> scan(c);
-        if (rank == 0 && t < head) {
-            const float v[1] = {to_float(x[t])};
-            scan.take(v, t);
-        }
+        Scan scan(c);
+        if (rank == 0 && t < head) scan.one(to_float(x[t]), Packed<T>::floor());
         int p = p0 + t;
         for (; p + (UNROLL - 1) * kBlock < p1; p += UNROLL * kBlock) {
-            P pk[UNROLL];
+            uint4 w[UNROLL];
 #pragma unroll
-            for (int i = 0; i < UNROLL; i++) pk[i] = load_pack(xp + p + i * kBlock);
+            for (int i = 0; i < UNROLL; i++) w[i] = __ldcs(xp + p + i * kBlock);
 #pragma unroll
-            for (int i = 0; i < UNROLL; i++) {
-                float v[VEC];
-#pragma unroll
-                for (int e = 0; e < VEC; e++) v[e] = to_float(pk[i].v[e]);
-                scan.take(v, head + (p + i * kBlock) * VEC);
-            }
+            for (int i = 0; i < UNROLL; i++) scan.template pack<T>(w[i]);
         }
-        for (; p < p1; p += kBlock) {
-            const P pk = load_pack(xp + p);
-            float v[VEC];
-#pragma unroll
-            for (int e = 0; e < VEC; e++) v[e] = to_float(pk.v[e]);
-            scan.take(v, head + p * VEC);
-        }
-        if (rank == ranks - 1 && t < vocab - tail0) {
-            const float v[1] = {to_float(x[tail0 + t])};
-            scan.take(v, tail0 + t);
-        }
+        for (; p < p1; p += kBlock) scan.template pack<T>(__ldcs(xp + p));
+        if (rank == ranks - 1 && t < vocab - tail0) scan.one(to_float(x[tail0 + t]), Packed<T>::floor());
 
-        const Sums mine = warp_join(Sums{scan.ref, scan.s0, scan.s1});
+        const Sums mine = warp_join(scan.sums());
         if (lane == 0) sums_s[warp] = mine;
-        uint64_t key = 0, list = 0;
+        uint32_t key = 0;
+        uint64_t bar = 0;
         if constexpr (TOP) {
-            if (scan.best > -INFINITY) {
-                int at = scan.best_at;  // the first of up to VEC values is the one of lowest index that equals the maximum
-                while (at + 1 < vocab && to_float(x[at]) != scan.best) at++;
-                key = rank_key(scan.best, uint32_t(at));
-            }
-            list = tournament(sort32(key, lane), list_s, lane, warp);
+            if (t == 0) n_streams = n_found = 0;
+            if (scan.best > -INFINITY) key = ordered(scan.best);
+            bar = uint64_t(bound_of(key, a.k, values_s, lane, warp)) << 32;  // 0: too few threads have a logit above -inf, all is looked at
         } else {
             __syncthreads();
         }
@@ -285,48 +345,41 @@ __global__ void __launch_bounds__(kBlock) logprobs_kernel(const T* __restrict__ 
         for (int w = 1; w < kLpWarps; w++) all = join(all, sums_s[w]);
 
         if constexpr (TOP) {
-            if (a.k > 1) {
-                uint64_t bar = list_s[0][a.k - 1];  // 0 where fewer than k threads have a logit above -inf: everything is looked at
-                while (true) {
-                    if (t == 0) n_streams = n_found = 0;
-                    __syncthreads();
-                    if (key >= bar || bar == 0) streams_s[atomicAdd(&n_streams, 1)] = t;
-                    __syncthreads();
-                    auto offer = [&](float v, int at) {
-                        const uint64_t k2 = rank_key(v, uint32_t(at));
-                        if (k2 < bar) return;
-                        const int place = atomicAdd(&n_found, 1);
-                        if (place < kCandidates) found_s[place] = k2;
-                    };
-                    const int streams = n_streams, per = (p1 - p0 + kBlock - 1) / kBlock;
-                    for (int i = t; i < streams * per; i += kBlock) {
-                        const int q = p0 + streams_s[i % streams] + (i / streams) * kBlock;
-                        if (q >= p1) continue;
-                        const P pk = xp[q];
+            while (true) {
+                if (uint64_t(key) << 32 >= (bar & 0xffffffff00000000ull)) streams_s[atomicAdd(&n_streams, 1)] = t;
+                __syncthreads();
+                auto offer = [&](float v, int at) {
+                    const uint64_t k2 = rank_key(v, uint32_t(at));
+                    if (k2 < bar) return;
+                    const int place = atomicAdd(&n_found, 1);
+                    if (place < kCandidates) found_s[place] = k2;
+                };
+                const int streams = n_streams, per = (p1 - p0 + kBlock - 1) / kBlock;
+                for (int i = t; i < streams * per; i += kBlock) {
+                    const int q = p0 + streams_s[i % streams] + (i / streams) * kBlock;
+                    if (q >= p1) continue;
+                    const uint4 w = xp[q];
+                    if (uint64_t(ordered(Packed<T>::top(w))) << 32 < (bar & 0xffffffff00000000ull)) continue;
+                    const T* v = reinterpret_cast<const T*>(&w);
 #pragma unroll
-                        for (int e = 0; e < VEC; e++) offer(to_float(pk.v[e]), head + q * VEC + e);
-                    }
-                    if (rank == 0 && t < head) offer(to_float(x[t]), t);
-                    if (rank == ranks - 1 && t < vocab - tail0) offer(to_float(x[tail0 + t]), tail0 + t);
-                    __syncthreads();
-                    const int found = n_found < kCandidates ? n_found : kCandidates;
-                    uint64_t best = 0;
-                    for (int i = warp * 32; i < found; i += kBlock) {
-                        const uint64_t part = sort32(i + lane < found ? found_s[i + lane] : 0, lane);
-                        best = i == warp * 32 ? part : merge32(best, part, lane);
-                    }
-                    const bool over = n_found > kCandidates;
-                    list = tournament(best, list_s, lane, warp);
-                    if (!over) break;
-                    bar = list_s[0][a.k - 1];  // the k-th largest of those that found room: a higher bar, and fewer above it
+                    for (int e = 0; e < VEC; e++) offer(to_float(v[e]), head + q * VEC + e);
                 }
+                if (rank == 0 && t < head) offer(to_float(x[t]), t);
+                if (rank == ranks - 1 && t < vocab - tail0) offer(to_float(x[tail0 + t]), tail0 + t);
+                __syncthreads();
+                const int n = n_found;
+                rank_keys(found_s, n < kCandidates ? n : kCandidates, a.k, list_s);
+                __syncthreads();
+                if (n <= kCandidates) break;
+                bar = list_s[a.k - 1];  // the k-th largest of those that found room: a higher bar, and fewer above it
+                if (t == 0) n_streams = n_found = 0;
+                __syncthreads();
             }
         }
         if (ranks > 1) {
             if (t == 0) block_s = all;
             ptx::cluster_sync();
             if (rank == 0) {
-                uint64_t other = 0;
                 for (int r = 1; r < ranks; r++) {
                     const uint32_t from = ptx::map_to_cta(ptx::smem_u32(&block_s), uint32_t(r));
                     Sums s;
@@ -335,20 +388,25 @@ __global__ void __launch_bounds__(kBlock) logprobs_kernel(const T* __restrict__ 
                     asm volatile("ld.shared::cluster.f32 %0, [%1+8];" : "=f"(s.s1) : "r"(from) : "memory");
                     all = join(all, s);
                 }
-                if constexpr (TOP) {
-                    if (warp < ranks) {
-                        const uint32_t from = ptx::map_to_cta(ptx::smem_u32(&list_s[0][lane]), uint32_t(warp));
-                        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(other) : "r"(from) : "memory");
+                if constexpr (TOP) {  // 32 lanes per rank: 8 ranks of up to 32 keys
+                    if (warp < ranks && lane < a.k) {
+                        const uint32_t from = ptx::map_to_cta(ptx::smem_u32(&list_s[lane]), uint32_t(warp));
+                        uint64_t k2;
+                        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(k2) : "r"(from) : "memory");
+                        found_s[warp * a.k + lane] = k2;
                     }
                 }
-                list = other;
             }
             ptx::cluster_sync();  // the other blocks' shared memory has been read
             if (rank != 0) continue;
-            if constexpr (TOP) list = tournament(list, list_s, lane, warp);
+            if constexpr (TOP) {
+                rank_keys(found_s, ranks * a.k, a.k, list_s);
+                __syncthreads();
+            }
         }
 
-        if (!(fabsf(all.s0) < INFINITY) || all.s0 == 0.f || !(fabsf(all.ref) < INFINITY)) {
+        // careful: no usable value, a NaN or +inf, or a maximum so near the floor that a value raised to it would count
+        if (!(fabsf(all.s0) < INFINITY) || !(fabsf(all.s1) < INFINITY) || all.s0 == 0.f || !(all.ref - Packed<T>::floor() * c >= 200.f)) {
             __syncthreads();
             row_carefully(x, a, row, red_s, &best_s);
             __syncthreads();
@@ -368,9 +426,9 @@ __global__ void __launch_bounds__(kBlock) logprobs_kernel(const T* __restrict__ 
             if (a.entropy) a.entropy[row] = (log_s0 - all.s1 / all.s0) * kLn2;
         }
         if constexpr (TOP) {
-            if (t < a.k) {  // k <= 32: one warp
-                a.top_ids[row * a.k + t] = key_index(list);
-                a.top_logp[row * a.k + t] = logp(key_value(list));
+            if (t < a.k) {
+                a.top_ids[row * a.k + t] = key_index(list_s[t]);
+                a.top_logp[row * a.k + t] = logp(key_value(list_s[t]));
             }
         }
         __syncthreads();  // the shared arrays are reused by the next row

@@ -27,90 +27,107 @@ struct RopeTensor {
     int heads;
 };
 
-// Blocks (x, y): block x takes tokens, block y a share of the token's units. The token's cosines and sines are worked out once per
-// block, while the first unit of every thread is on its way, and serve all heads. A unit is VEC pairs, i.e. two runs of VEC
-// elements: VEC apart by rotary / 2 in the half layout, next to each other otherwise and in the part that is only copied.
+// Blocks (x, y): block x takes tokens, block y a share of the token's units. A unit is VEC pairs, i.e. two runs of VEC elements:
+// rotary / 2 apart in the half layout, next to each other otherwise and in the part that is only copied. A thread has up to two units
+// and asks for both before the token's cosines and sines are worked out, once per block, for all heads.
+constexpr int kRopeUnits = 2, kRopeThreads = 256;
+
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) rope_kernel(RopeTensor q, RopeTensor k, RopeTensor v, RopeArgs a) {
+__global__ void __launch_bounds__(kRopeThreads) rope_kernel(RopeTensor q, RopeTensor k, RopeTensor v, RopeArgs a) {
     using P = Pack<T, VEC>;
     extern __shared__ float2 turn_s[];  // cosine and sine of each pair, times mscale
     __shared__ int64_t place_s[2];      // page (-1: nothing is written) and place of the token
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
-    const int half = int(a.rotary / 2), D = int(a.D), turned = half / VEC;
+    const int half = int(a.rotary / 2), D = int(a.D), turned = half / VEC, threads = int(blockDim.x);
     const int per_head = turned + (D - int(a.rotary) + 2 * VEC - 1) / (2 * VEC);
-    const int units = (q.heads + k.heads + v.heads) * per_head, step = 256 * gridDim.y;
-    const int first = int(blockIdx.y) * 256 + int(threadIdx.x);
+    const int units = (q.heads + k.heads + v.heads) * per_head, pass = threads * kRopeUnits;
     for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
-        P x0, x1;
-        const RopeTensor* of;
-        int h, u, d0, d1;
-        auto fetch = [&](int w) {
-            h = w / per_head;
-            u = w - h * per_head;
-            of = &q;
-            if (h >= q.heads) {
-                h -= q.heads;
-                of = &k;
-                if (h >= k.heads) {
-                    h -= k.heads;
-                    of = &v;
-                }
-            }
-            if (u >= turned) {
-                d0 = int(a.rotary) + (u - turned) * 2 * VEC;
-                d1 = d0 + VEC;
-            } else {
-                d0 = a.interleaved ? u * 2 * VEC : u * VEC;
-                d1 = a.interleaved ? d0 + VEC : d0 + half;
-            }
-            const T* in = static_cast<const T*>(of->in) + t * of->in_t + h * of->in_h;
-            x0 = load_pack(reinterpret_cast<const P*>(in + d0));
-            if (VEC > 1 || d1 < D) x1 = load_pack(reinterpret_cast<const P*>(in + d1));
-        };
-        if (first < units) fetch(first);
-        for (int i = threadIdx.x; i < half; i += 256) {
-            const double turns = double(a.positions[t]) * (a.inv_freq[i] * 0.15915494309189533577);
-            float c, s;
-            sincospif(2.f * float(turns - rint(turns)), &s, &c);
-            turn_s[i] = make_float2(a.mscale * c, a.mscale * a.sign * s);
-        }
-        if (a.slots && threadIdx.x == 255) {
-            const int64_t slot = a.slots[t];
-            const int64_t page = slot < 0 ? -1 : slot / a.page_size;
-            if (page >= a.num_pages) report_bad_index(a.status, kIndexSlot);
-            place_s[0] = page < a.num_pages ? page : -1;
-            place_s[1] = slot - page * a.page_size;
-        }
-        __syncthreads();
-        for (int w = first; w < units; w += step) {
-            if (w != first) fetch(w);
-            const bool cached = of != &q;
-            if (cached && place_s[0] < 0) continue;
-            T* out = static_cast<T*>(of->out) + (cached ? place_s[0] * of->out_t + place_s[1] * of->out_s : t * of->out_t) + h * of->out_h;
-            if (u < turned && of != &v) {
-                if (a.interleaved) {
+        bool ready = false;
+        for (int base = int(blockIdx.y) * pass; base < units; base += pass * int(gridDim.y)) {
+            P x0[kRopeUnits], x1[kRopeUnits];
+            int which[kRopeUnits], unit[kRopeUnits], d0[kRopeUnits], d1[kRopeUnits];
+            int64_t out_at[kRopeUnits];
 #pragma unroll
-                    for (int e = 0; e < 2 * VEC; e += 2) {
-                        const float2 cs = turn_s[u * VEC + e / 2];
-                        T& e0 = e < VEC ? x0.v[e] : x1.v[e - VEC];
-                        T& e1 = e + 1 < VEC ? x0.v[e + 1 < VEC ? e + 1 : 0] : x1.v[e + 1 - VEC];
-                        const float f0 = to_float(e0), f1 = to_float(e1);
-                        e0 = from_float<T>(f0 * cs.x - f1 * cs.y);
-                        e1 = from_float<T>(f1 * cs.x + f0 * cs.y);
-                    }
+            for (int j = 0; j < kRopeUnits; j++) {
+                const int w = base + j * threads + int(threadIdx.x);
+                which[j] = -1;
+                if (w >= units) continue;
+                int h = w / per_head;
+                const int u = w - h * per_head;
+                const bool is_q = h < q.heads, is_v = h >= q.heads + k.heads;
+                which[j] = is_q ? 0 : is_v ? 2 : 1;
+                h -= is_q ? 0 : is_v ? q.heads + k.heads : q.heads;
+                unit[j] = u;
+                if (u >= turned) {
+                    d0[j] = int(a.rotary) + (u - turned) * 2 * VEC;
+                    d1[j] = d0[j] + VEC;
                 } else {
+                    d0[j] = a.interleaved ? u * 2 * VEC : u * VEC;
+                    d1[j] = a.interleaved ? d0[j] + VEC : d0[j] + half;
+                }
+                const T* in = static_cast<const T*>(is_q ? q.in : is_v ? v.in : k.in) +
+                              t * (is_q ? q.in_t : is_v ? v.in_t : k.in_t) + h * (is_q ? q.in_h : is_v ? v.in_h : k.in_h);
+                out_at[j] = h * (is_q ? q.out_h : is_v ? v.out_h : k.out_h);
+                x0[j] = load_pack(reinterpret_cast<const P*>(in + d0[j]));
+                if (VEC > 1 || d1[j] < D) x1[j] = load_pack(reinterpret_cast<const P*>(in + d1[j]));
+            }
+            if (!ready) {
+                ready = true;
+                for (int i = threadIdx.x; i < half; i += threads) {
+                    const double turns = double(a.positions[t]) * (a.inv_freq[i] * 0.15915494309189533577);
+                    float c, s;
+                    sincospif(2.f * float(turns - rint(turns)), &s, &c);
+                    turn_s[i] = make_float2(a.mscale * c, a.mscale * a.sign * s);
+                }
+                if (a.slots && int(threadIdx.x) == threads - 1) {
+                    const int64_t slot = a.slots[t];
+                    // a cache of 2^32 places or more takes the long division
+                    const int64_t page = slot < 0 ? -1
+                                         : ((slot | a.page_size) >> 32) == 0 ? int64_t(uint32_t(slot) / uint32_t(a.page_size))
+                                                                             : slot / a.page_size;
+                    if (page >= a.num_pages) report_bad_index(a.status, kIndexSlot);
+                    place_s[0] = page < a.num_pages ? page : -1;
+                    place_s[1] = slot - page * a.page_size;
+                }
+                __syncthreads();
+            }
 #pragma unroll
-                    for (int e = 0; e < VEC; e++) {
-                        const float2 cs = turn_s[u * VEC + e];
-                        const float f0 = to_float(x0.v[e]), f1 = to_float(x1.v[e]);
-                        x0.v[e] = from_float<T>(f0 * cs.x - f1 * cs.y);
-                        x1.v[e] = from_float<T>(f1 * cs.x + f0 * cs.y);
+            for (int j = 0; j < kRopeUnits; j++) {
+                if (which[j] < 0) continue;
+                T* out;
+                if (which[j] == 0) {
+                    out = static_cast<T*>(q.out) + t * q.out_t + out_at[j];
+                } else {
+                    if (place_s[0] < 0) continue;
+                    const bool is_v = which[j] == 2;
+                    out = static_cast<T*>(is_v ? v.out : k.out) + place_s[0] * (is_v ? v.out_t : k.out_t) +
+                          place_s[1] * (is_v ? v.out_s : k.out_s) + out_at[j];
+                }
+                if (unit[j] < turned && which[j] != 2) {
+                    T e[2 * VEC];
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) {
+                        e[i] = x0[j].v[i];
+                        e[VEC + i] = x1[j].v[i];
+                    }
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) {
+                        const float2 cs = turn_s[unit[j] * VEC + i];
+                        const float f0 = to_float(a.interleaved ? e[2 * i] : e[i]), f1 = to_float(a.interleaved ? e[2 * i + 1] : e[VEC + i]);
+                        const T y0 = from_float<T>(f0 * cs.x - f1 * cs.y), y1 = from_float<T>(f1 * cs.x + f0 * cs.y);
+                        if (a.interleaved) {
+                            (2 * i < VEC ? x0[j].v[2 * i < VEC ? 2 * i : 0] : x1[j].v[2 * i < VEC ? 0 : 2 * i - VEC]) = y0;
+                            (2 * i + 1 < VEC ? x0[j].v[2 * i + 1 < VEC ? 2 * i + 1 : 0] : x1[j].v[2 * i + 1 < VEC ? 0 : 2 * i + 1 - VEC]) = y1;
+                        } else {
+                            x0[j].v[i] = y0;
+                            x1[j].v[i] = y1;
+                        }
                     }
                 }
+                *reinterpret_cast<P*>(out + d0[j]) = x0[j];
+                if (VEC > 1 || d1[j] < D) *reinterpret_cast<P*>(out + d1[j]) = x1[j];
             }
-            *reinterpret_cast<P*>(out + d0) = x0;
-            if (VEC > 1 || d1 < D) *reinterpret_cast<P*>(out + d1) = x1;
         }
         __syncthreads();  // turn_s and place_s are the next token's
     }
@@ -120,13 +137,16 @@ template <typename T, int VEC>
 int launch_rope(Ctx* ctx, const RopeTensor& q, const RopeTensor& k, const RopeTensor& v, const RopeArgs& a) {
     const int64_t per_head = a.rotary / 2 / VEC + ceil_div(a.D - a.rotary, 2 * VEC);
     const int64_t units = (int64_t(q.heads) + k.heads + v.heads) * per_head;
-    // few tokens: a unit per thread; many: a block per token, so that its angles are worked out once
-    const int64_t shares = ceil_div(units, 256);
+    // few tokens: enough blocks per token that a thread has one round of units; many: a block per token, so that its angles are worked
+    // out once (8192 tokens of 384 units: 75 us with three blocks per token, 37 with one)
+    int64_t threads = ceil_div(ceil_div(units, kRopeUnits), 32) * 32;
+    if (threads > kRopeThreads) threads = kRopeThreads;
+    const int64_t shares = ceil_div(units, threads * kRopeUnits);
     const int64_t y = a.tokens * shares <= 2 * int64_t(ctx->sm_count) ? shares : 1;
     const int64_t cap = int64_t(1) << 20;
     const size_t smem = size_t(a.rotary / 2) * sizeof(float2);
-    DOCC_CUDA_TRY(launch_pdl(rope_kernel<T, VEC>, dim3(unsigned(a.tokens < cap ? a.tokens : cap), unsigned(y)), dim3(256), smem, ctx->stream, q, k,
-                             v, a));
+    DOCC_CUDA_TRY(launch_pdl(rope_kernel<T, VEC>, dim3(unsigned(a.tokens < cap ? a.tokens : cap), unsigned(y)), dim3(unsigned(threads)), smem,
+                             ctx->stream, q, k, v, a));
     return after_launch(ctx, "rope_kernel");
 }
 
