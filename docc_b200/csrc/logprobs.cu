@@ -7,7 +7,7 @@
 // it is raised when a value lies 16 above it, so that in practice nothing is rescaled after a thread's first values.
 //
 // The alternatives cost no second pass. A thread keeps its largest logit; T, a value that at least k threads' maxima reach, is a lower
-// bound of the row's k-th largest, and only those threads can hold others: some thirty of 256 for k = 20. Their logits are read again
+// bound of the row's k-th largest, and only those threads can hold others: some thirty of 512 for k = 20. Their logits are read again
 // (from L2), and what reaches T, few more than k values, is ranked by counting.
 //
 // With fewer rows than fill the machine, a cluster of up to eight blocks takes a row; the other blocks' sums and lists meet in the first
@@ -20,8 +20,7 @@ namespace docc_b200 {
 namespace {
 
 constexpr int kMaxTop = 32;
-constexpr int kBlock = 256, kLpWarps = kBlock / 32;
-constexpr int kCandidates = 1024;
+constexpr int kCandidates = 1024, kRescan = 4;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // Order of the alternatives: larger logit first, then the lower index; a NaN is above everything. -0 and +0 are equal. No key is 0.
@@ -64,7 +63,7 @@ __device__ __forceinline__ float block_max_f(float v, float* smem) {
     if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = v;
     __syncthreads();
     float r = smem[0];
-    for (int w = 1; w < kLpWarps; w++) r = fmaxf(r, smem[w]);
+    for (int w = 1; w < int(blockDim.x >> 5); w++) r = fmaxf(r, smem[w]);
     return r;
 }
 
@@ -72,10 +71,10 @@ __device__ __forceinline__ float block_max_f(float v, float* smem) {
 // fp32's range (a row of the type's lowest value). The row is read once for the maximum, once for the sums and once per alternative.
 template <typename T> __device__ __noinline__ void row_carefully(const T* x, const LogpArgs& a, int64_t row, float* red, unsigned long long* best) {
     float m = -INFINITY;
-    for (int64_t c = threadIdx.x; c < a.vocab; c += kBlock) m = fmaxf(m, to_float(x[c]));
+    for (int64_t c = threadIdx.x; c < a.vocab; c += blockDim.x) m = fmaxf(m, to_float(x[c]));
     m = block_max_f(m, red);
     float s0 = 0.f, s1 = 0.f;
-    for (int64_t c = threadIdx.x; c < a.vocab; c += kBlock) {
+    for (int64_t c = threadIdx.x; c < a.vocab; c += blockDim.x) {
         const float d = (to_float(x[c]) - m) * a.scale, e = expf(d);
         s0 += e;
         s1 += e == 0.f ? 0.f : d * e;
@@ -95,7 +94,7 @@ template <typename T> __device__ __noinline__ void row_carefully(const T* x, con
         if (threadIdx.x == 0) *best = 0;
         __syncthreads();
         unsigned long long mine = 0;
-        for (int64_t c = threadIdx.x; c < a.vocab; c += kBlock) {
+        for (int64_t c = threadIdx.x; c < a.vocab; c += blockDim.x) {
             const unsigned long long key = rank_key(to_float(x[c]), uint32_t(c));
             if ((key < last || i == 0) && key > mine) mine = key;
         }
@@ -114,26 +113,22 @@ template <typename T> __device__ __noinline__ void row_carefully(const T* x, con
 struct Sums {
     float ref, s0, s1;  // reference and sums in units of log 2
 };
-// Sums against the larger of two references; without values (s0 = 0) a reference counts as -inf.
-__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
-    const float ra = a.s0 == 0.f ? -INFINITY : a.ref, rb = b.s0 == 0.f ? -INFINITY : b.ref;
-    Sums r;
-    r.ref = fmaxf(ra, rb);
-    if (r.ref == -INFINITY) return Sums{0.f, 0.f, 0.f};
-    const float da = fmaxf(ra - r.ref, -200.f), db = fmaxf(rb - r.ref, -200.f);  // 2^-200 is 0: nothing is left of that side
-    const float fa = lp_ex2(da), fb = lp_ex2(db);
-    r.s0 = a.s0 * fa + b.s0 * fb;
-    r.s1 = fmaf(a.s0, da, a.s1) * fa + fmaf(b.s0, db, b.s1) * fb;
-    return r;
-}
-__device__ __forceinline__ Sums warp_join(Sums v) {
+// The sums of N lanes (a power of two, the same ones for every lane of a group) against the largest of their references. A side without
+// values (s0 = 0) counts as -inf. The order of the additions is that of the lanes.
+template <int N> __device__ __forceinline__ Sums join_lanes(const Sums& v) {
+    const float own = v.s0 == 0.f ? -INFINITY : v.ref;
+    float top = own;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        // lanes o apart swap: the lower one's sums come first on both sides, so both get the same bits
-        const Sums w{__shfl_xor_sync(0xffffffffu, v.ref, o), __shfl_xor_sync(0xffffffffu, v.s0, o), __shfl_xor_sync(0xffffffffu, v.s1, o)};
-        v = (threadIdx.x & o) ? join(w, v) : join(v, w);
+    for (int o = N / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (top == -INFINITY) top = 0.f;
+    const float d = fmaxf(own - top, -200.f), f = lp_ex2(d);  // 2^-200 is 0: nothing is left of that side
+    Sums r{top, v.s0 * f, fmaf(v.s0, d, v.s1) * f};
+#pragma unroll
+    for (int o = N / 2; o > 0; o >>= 1) {
+        r.s0 += __shfl_xor_sync(0xffffffffu, r.s0, o);
+        r.s1 += __shfl_xor_sync(0xffffffffu, r.s1, o);
     }
-    return v;
+    return r;
 }
 
 constexpr float kHeadroom = 16.f;
@@ -202,6 +197,17 @@ template <> struct Packed<__half> {
     }
 };
 
+// Where in a pack of N values the first one equal to v stands (N - 1 if none is).
+template <typename T> __device__ __forceinline__ int first_of(const uint4& w, float v) {
+    constexpr int N = 16 / sizeof(T);
+    const T* x = reinterpret_cast<const T*>(&w);
+    int at = N - 1;
+#pragma unroll
+    for (int e = N - 2; e >= 0; e--)
+        if (to_float(x[e]) == v) at = e;
+    return at;
+}
+
 struct Scan {
     float c;           // scale log2 e
     float ref, limit;  // limit: the logit whose multiple by c lies kHeadroom above ref
@@ -258,8 +264,8 @@ __device__ __forceinline__ uint32_t ordered(float x) { return uint32_t(rank_key(
 
 // A value (as ordered bits) that at least k of the block's threads reach with theirs, near the k-th largest: a warp's j-th largest,
 // j = ceil(k / warps), of the r-th best warp, j r >= k. `values_s` has room for one word per warp. 0 if there is none.
-__device__ __forceinline__ uint32_t bound_of(uint32_t mine, int k, uint32_t* values_s, int lane, int warp) {
-    const int j = (k + kLpWarps - 1) / kLpWarps, r = (k + j - 1) / j;
+template <int WARPS> __device__ __forceinline__ uint32_t bound_of(uint32_t mine, int k, uint32_t* values_s, int lane, int warp) {
+    const int j = (k + WARPS - 1) / WARPS, r = (k + j - 1) / j;
     uint32_t rest = mine, nth = 0;
     for (int i = 0; i < j; i++) {
         nth = __reduce_max_sync(0xffffffffu, rest);
@@ -267,112 +273,140 @@ __device__ __forceinline__ uint32_t bound_of(uint32_t mine, int k, uint32_t* val
     }
     if (lane == 0) values_s[warp] = nth;
     __syncthreads();
-    const uint32_t v = lane < kLpWarps ? values_s[lane] : 0;
+    const uint32_t v = lane < WARPS ? values_s[lane] : 0;
     int above = 0;
 #pragma unroll
-    for (int w = 0; w < kLpWarps; w++) {
+    for (int w = 0; w < WARPS; w++) {
         const uint32_t o = __shfl_sync(0xffffffffu, v, w);
         above += o > v || (o == v && w < lane);
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, lane < kLpWarps && above == r - 1);
+    const unsigned hit = __ballot_sync(0xffffffffu, lane < WARPS && above == r - 1);
     return __shfl_sync(0xffffffffu, v, __ffs(hit) - 1);
 }
-// The k largest of n distinct keys, in order: a key's place is the number of keys above it. Places past the last key hold 0.
+// The k largest of n distinct keys, in order: a key's place is the number of keys above it, counted by a thread per key (a ballot of
+// 32 comparisons per step has fewer instructions and takes twice as long: each step waits for the one before). Places past the last
+// key hold 0.
 __device__ __forceinline__ void rank_keys(const uint64_t* keys, int n, int k, uint64_t* out) {
     if (int(threadIdx.x) < k && int(threadIdx.x) >= n) out[threadIdx.x] = 0;
-    for (int i = threadIdx.x; i < n; i += kBlock) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
         const uint64_t mine = keys[i];
         int above = 0;
-#pragma unroll 4
+#pragma unroll 8
         for (int j = 0; j < n; j++) above += keys[j] > mine;
         if (above < k && mine != 0) out[above] = mine;
     }
 }
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(kBlock) logprobs_kernel(const T* __restrict__ X, LogpArgs a, int ranks) {
-    constexpr int VEC = 16 / sizeof(T), UNROLL = 4;
-    __shared__ Sums sums_s[kLpWarps];
-    __shared__ float red_s[kLpWarps];
-    __shared__ uint32_t values_s[kLpWarps];
+// BLOCK: 256 threads without alternatives, where nothing but the stream counts (141 us for 4096 rows of 50021 fp32, with 512: 153); 512
+// with them, since what follows the stream takes a block's time whatever its size (256 rows of 128000: 20.3 us, with 256: 25.8).
+template <typename T, bool TOP, int BLOCK>
+__global__ void __launch_bounds__(BLOCK, 1024 / BLOCK) logprobs_kernel(const T* __restrict__ X, LogpArgs a, int log_ranks) {
+    constexpr int VEC = 16 / sizeof(T), UNROLL = 4, WARPS = BLOCK / 32;
+    __shared__ Sums sums_s[WARPS];
+    __shared__ float red_s[WARPS];
+    __shared__ uint32_t values_s[WARPS];
     __shared__ unsigned long long best_s;
     __shared__ uint64_t list_s[kMaxTop];
     __shared__ uint64_t found_s[TOP ? kCandidates : 1];
-    __shared__ int streams_s[TOP ? kBlock : 1];
-    __shared__ int n_streams, n_found;
+    __shared__ int streams_s[TOP ? BLOCK : 1];
+    __shared__ int hits_s[TOP ? kCandidates : 1];
+    __shared__ int n_streams, n_found, n_hits;
     __shared__ Sums block_s;  // read, like list_s, by the cluster's first block
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const int rank = int(blockIdx.x % ranks);
+    const int ranks = 1 << log_ranks, rank = int(blockIdx.x) & (ranks - 1);
     const float c = a.scale * kLog2e;
-    for (int64_t row = blockIdx.x / ranks; row < a.rows; row += gridDim.x / ranks) {
+    for (int64_t row = blockIdx.x >> log_ranks; row < a.rows; row += gridDim.x >> log_ranks) {
         const T* x = X + row * a.ldx;
         const int vocab = int(a.vocab);
         // values before the first 16-byte boundary, whole packs, values behind the last
         int head = int((16 - reinterpret_cast<uintptr_t>(x) % 16) % 16 / sizeof(T));
         if (head > vocab) head = vocab;
         const int packs = (vocab - head) / VEC, tail0 = head + packs * VEC;
-        const int p0 = int(int64_t(packs) * rank / ranks), p1 = int(int64_t(packs) * (rank + 1) / ranks);
+        const int share = (packs + ranks - 1) >> log_ranks, p0 = min(rank * share, packs), p1 = min(p0 + share, packs);
         const uint4* xp = reinterpret_cast<const uint4*>(x + head);
+
+        // asked for now, used at the end
+        const int64_t id = rank == 0 && t == 0 && a.logp ? a.ids[row] : -1;
+        const float chosen = id >= 0 && id < a.vocab ? to_float(x[id]) : NAN;
 
         Scan scan(c);
         if (rank == 0 && t < head) scan.one(to_float(x[t]), Packed<T>::floor());
         int p = p0 + t;
-        for (; p + (UNROLL - 1) * kBlock < p1; p += UNROLL * kBlock) {
+        for (; p + (UNROLL - 1) * BLOCK < p1; p += UNROLL * BLOCK) {
             uint4 w[UNROLL];
 #pragma unroll
-            for (int i = 0; i < UNROLL; i++) w[i] = __ldcs(xp + p + i * kBlock);
+            for (int i = 0; i < UNROLL; i++) w[i] = __ldcs(xp + p + i * BLOCK);
 #pragma unroll
             for (int i = 0; i < UNROLL; i++) scan.template pack<T>(w[i]);
         }
-        for (; p < p1; p += kBlock) scan.template pack<T>(__ldcs(xp + p));
+        for (; p < p1; p += BLOCK) scan.template pack<T>(__ldcs(xp + p));
         if (rank == ranks - 1 && t < vocab - tail0) scan.one(to_float(x[tail0 + t]), Packed<T>::floor());
 
-        const Sums mine = warp_join(scan.sums());
+        const Sums mine = join_lanes<32>(scan.sums());
         if (lane == 0) sums_s[warp] = mine;
         uint32_t key = 0;
         uint64_t bar = 0;
         if constexpr (TOP) {
-            if (t == 0) n_streams = n_found = 0;
+            if (t == 0) n_streams = n_found = n_hits = 0;
             if (scan.best > -INFINITY) key = ordered(scan.best);
-            bar = uint64_t(bound_of(key, a.k, values_s, lane, warp)) << 32;  // 0: too few threads have a logit above -inf, all is looked at
+            bar = uint64_t(bound_of<WARPS>(key, a.k, values_s, lane, warp)) << 32;  // 0: too few threads have a logit above -inf, all is looked at
         } else {
             __syncthreads();
         }
-        Sums all = sums_s[0];
-#pragma unroll
-        for (int w = 1; w < kLpWarps; w++) all = join(all, sums_s[w]);
+        Sums all = join_lanes<WARPS>(sums_s[lane % WARPS]);
 
         if constexpr (TOP) {
             while (true) {
-                if (uint64_t(key) << 32 >= (bar & 0xffffffff00000000ull)) streams_s[atomicAdd(&n_streams, 1)] = t;
+                if (key >= uint32_t(bar >> 32)) streams_s[atomicAdd(&n_streams, 1)] = t;
                 __syncthreads();
-                auto offer = [&](float v, int at) {
-                    const uint64_t k2 = rank_key(v, uint32_t(at));
-                    if (k2 < bar) return;
-                    const int place = atomicAdd(&n_found, 1);
-                    if (place < kCandidates) found_s[place] = k2;
-                };
-                const int streams = n_streams, per = (p1 - p0 + kBlock - 1) / kBlock;
-                for (int i = t; i < streams * per; i += kBlock) {
-                    const int q = p0 + streams_s[i % streams] + (i / streams) * kBlock;
-                    if (q >= p1) continue;
-                    const uint4 w = xp[q];
-                    if (uint64_t(ordered(Packed<T>::top(w))) << 32 < (bar & 0xffffffff00000000ull)) continue;
-                    const T* v = reinterpret_cast<const T*>(&w);
+                // a warp per stream, a pack per lane; packs that hold something are queued
+                const int streams = n_streams, per = (p1 - p0 + BLOCK - 1) / BLOCK;
+                for (int j = lane; j < (per + 31) / 32 * 32; j += 32) {
+                    for (int s0 = warp; s0 < streams; s0 += WARPS * kRescan) {
+                        uint4 w[kRescan];
+                        int q[kRescan];
 #pragma unroll
-                    for (int e = 0; e < VEC; e++) offer(to_float(v[e]), head + q * VEC + e);
+                        for (int h = 0; h < kRescan; h++) {  // all of a round are asked for together
+                            const int s = s0 + h * WARPS;
+                            q[h] = s < streams ? p0 + streams_s[s] + j * BLOCK : p1;
+                            if (q[h] < p1) w[h] = xp[q[h]];
+                        }
+#pragma unroll
+                        for (int h = 0; h < kRescan; h++) {
+                            if (q[h] >= p1) continue;
+                            const float top = Packed<T>::top(w[h]);
+                            const uint32_t value = ordered(top);
+                            if (value < uint32_t(bar >> 32)) continue;
+                            // of equal values only those up to the bar's index: what is queued holds a key that reaches the bar
+                            if (value == uint32_t(bar >> 32) && rank_key(top, uint32_t(head + q[h] * VEC + first_of<T>(w[h], top))) < bar) continue;
+                            const int place = atomicAdd(&n_hits, 1);
+                            if (place < kCandidates) hits_s[place] = q[h];
+                        }
+                    }
                 }
-                if (rank == 0 && t < head) offer(to_float(x[t]), t);
-                if (rank == ranks - 1 && t < vocab - tail0) offer(to_float(x[tail0 + t]), tail0 + t);
                 __syncthreads();
-                const int n = n_found;
+                const int hits = n_hits < kCandidates ? n_hits : kCandidates, edges = (rank == 0 ? head : 0) + (rank == ranks - 1 ? vocab - tail0 : 0);
+                for (int i = t; i < hits * VEC + edges; i += BLOCK) {
+                    int at;
+                    if (i < hits * VEC) at = head + hits_s[i / VEC] * VEC + i % VEC;
+                    else at = i - hits * VEC < (rank == 0 ? head : 0) ? i - hits * VEC : tail0 + (i - hits * VEC - (rank == 0 ? head : 0));
+                    const uint64_t k2 = rank_key(to_float(x[at]), uint32_t(at));
+                    if (k2 >= bar) {
+                        const int place = atomicAdd(&n_found, 1);
+                        if (place < kCandidates) found_s[place] = k2;
+                    }
+                }
+                __syncthreads();
+                const int n = n_found, queued = n_hits;
                 rank_keys(found_s, n < kCandidates ? n : kCandidates, a.k, list_s);
                 __syncthreads();
-                if (n <= kCandidates) break;
-                bar = list_s[a.k - 1];  // the k-th largest of those that found room: a higher bar, and fewer above it
-                if (t == 0) n_streams = n_found = 0;
+                if (n <= kCandidates && queued <= kCandidates) break;
+                // more than found room: those that did are kCandidates keys or more that reach the bar, and all but k of them lie below
+                // their k-th largest, the next bar, so every round leaves hundreds fewer above it
+                bar = list_s[a.k - 1];
+                if (t == 0) n_streams = n_found = n_hits = 0;
                 __syncthreads();
             }
         }
@@ -380,14 +414,14 @@ __global__ void __launch_bounds__(kBlock) logprobs_kernel(const T* __restrict__ 
             if (t == 0) block_s = all;
             ptx::cluster_sync();
             if (rank == 0) {
-                for (int r = 1; r < ranks; r++) {
-                    const uint32_t from = ptx::map_to_cta(ptx::smem_u32(&block_s), uint32_t(r));
-                    Sums s;
+                Sums s{0.f, 0.f, 0.f};
+                if (lane < ranks) {
+                    const uint32_t from = ptx::map_to_cta(ptx::smem_u32(&block_s), uint32_t(lane));
                     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(s.ref) : "r"(from) : "memory");
                     asm volatile("ld.shared::cluster.f32 %0, [%1+4];" : "=f"(s.s0) : "r"(from) : "memory");
                     asm volatile("ld.shared::cluster.f32 %0, [%1+8];" : "=f"(s.s1) : "r"(from) : "memory");
-                    all = join(all, s);
                 }
+                all = join_lanes<32>(s);
                 if constexpr (TOP) {  // 32 lanes per rank: 8 ranks of up to 32 keys
                     if (warp < ranks && lane < a.k) {
                         const uint32_t from = ptx::map_to_cta(ptx::smem_u32(&list_s[lane]), uint32_t(warp));
@@ -419,10 +453,7 @@ __global__ void __launch_bounds__(kBlock) logprobs_kernel(const T* __restrict__ 
             return r == -INFINITY && v > -INFINITY ? v * a.scale - (all.ref + log_s0) * kLn2 : r;
         };
         if (t == 0) {
-            if (a.logp) {
-                const int64_t id = a.ids[row];
-                a.logp[row] = id < 0 || id >= a.vocab ? NAN : logp(to_float(x[id]));
-            }
+            if (a.logp) a.logp[row] = logp(chosen);  // of a NaN where there is no such token
             if (a.entropy) a.entropy[row] = (log_s0 - all.s1 / all.s0) * kLn2;
         }
         if constexpr (TOP) {
@@ -437,13 +468,18 @@ __global__ void __launch_bounds__(kBlock) logprobs_kernel(const T* __restrict__ 
 
 template <typename T, bool TOP>
 int launch_logprobs(Ctx* ctx, const void* X, const LogpArgs& a) {
-    int ranks = 1;
-    while (ranks < 8 && a.rows * ranks < int64_t(ctx->sm_count) * 2 && a.vocab / (2 * ranks) >= 2048) ranks *= 2;
+    constexpr int BLOCK = TOP ? 512 : 256;
+    // clusters only while every block has an SM of its own: at 256 rows two blocks per row took 29 us instead of 20, eight took 53
+    int ranks = 1, log_ranks = 0;
+    while (ranks < 8 && a.rows * ranks * 2 <= ctx->sm_count && a.vocab / (2 * ranks) >= 2048) {
+        ranks *= 2;
+        log_ranks++;
+    }
     const int64_t cap = int64_t(1) << 20;  // rows beyond it are taken in turn
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(unsigned((a.rows < cap ? a.rows : cap) * ranks));
-    cfg.blockDim = dim3(kBlock);
+    cfg.blockDim = dim3(BLOCK);
     cfg.stream = ctx->stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -453,7 +489,7 @@ int launch_logprobs(Ctx* ctx, const void* X, const LogpArgs& a) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = ranks > 1 ? 2 : 1;
-    DOCC_CUDA_TRY(cudaLaunchKernelEx(&cfg, logprobs_kernel<T, TOP>, static_cast<const T*>(X), a, ranks));
+    DOCC_CUDA_TRY(cudaLaunchKernelEx(&cfg, logprobs_kernel<T, TOP, BLOCK>, static_cast<const T*>(X), a, log_ranks));
     return after_launch(ctx, "logprobs_kernel");
 }
 template <typename T>

@@ -14,7 +14,7 @@ namespace docc_b200 {
 namespace {
 
 constexpr int64_t kRmsMaxCols = 32768;  // the row is staged in shared memory in fp32: 128 KB of 227
-constexpr int kRmsGroup = 128;
+constexpr int kRmsGroup = 128, kRmsLoads = 8;
 constexpr float kE4m3Max = 448.f;
 
 // Maximum that keeps a NaN, so that a group holding one gets a NaN scale instead of a plausible one.
@@ -187,13 +187,25 @@ __global__ void __launch_bounds__(256) rmsnorm_row_kernel(const T* X, const T* R
         const T* x = X + row * a.ldx;
         const T* r = R ? R + row * a.ldr : nullptr;
         float ss = 0.f;
-#pragma unroll 8
-        for (int c = t; c < cols; c += 256) {
-            float v = to_float(x[c]);
-            if (r) v += to_float(r[c]);
-            row_s[c] = v;
-            if (S) S[row * a.cols + c] = from_float<T>(v);
-            ss = fmaf(v, v, ss);
+        for (int c0 = t; c0 < cols; c0 += 256 * kRmsLoads) {  // all loads of a round before the first use
+            T vx[kRmsLoads], vr[kRmsLoads];
+#pragma unroll
+            for (int i = 0; i < kRmsLoads; i++)
+                if (c0 + i * 256 < cols) vx[i] = x[c0 + i * 256];
+            if (r) {
+#pragma unroll
+                for (int i = 0; i < kRmsLoads; i++)
+                    if (c0 + i * 256 < cols) vr[i] = r[c0 + i * 256];
+            }
+#pragma unroll
+            for (int i = 0; i < kRmsLoads; i++) {
+                const int c = c0 + i * 256;
+                if (c >= cols) break;
+                const float v = r ? to_float(vx[i]) + to_float(vr[i]) : to_float(vx[i]);
+                row_s[c] = v;
+                if (S) S[row * a.cols + c] = from_float<T>(v);
+                ss = fmaf(v, v, ss);
+            }
         }
         const float rstd = rsqrtf(block_sum_f(ss, red) / float(cols) + a.eps);
         if constexpr (!Q8) {

@@ -28,28 +28,66 @@ struct RopeTensor {
 };
 
 // Blocks (x, y): block x takes tokens, block y a share of the token's units. A unit is VEC pairs, i.e. two runs of VEC elements:
-// rotary / 2 apart in the half layout, next to each other otherwise and in the part that is only copied. A thread has up to two units
-// and asks for both before the token's cosines and sines are worked out, once per block, for all heads.
-constexpr int kRopeUnits = 2, kRopeThreads = 256;
+// rotary / 2 apart in the half layout, next to each other otherwise and in the part that is only copied. A thread has up to UNITS units
+// and asks for all of them before the token's cosines and sines are worked out, once per block, for all heads.
+constexpr int kRopeThreads = 256;
 
-template <typename T, int VEC>
+// Elements 2i and 2i + 1 of a run as fp32, and back (rounded once).
+template <typename T> __device__ __forceinline__ float2 get2(const T* x) { return make_float2(to_float(x[0]), to_float(x[1])); }
+template <> __device__ __forceinline__ float2 get2<__half>(const __half* x) { return __half22float2(*reinterpret_cast<const __half2*>(x)); }
+template <typename T> __device__ __forceinline__ void put2(T* x, float a, float b) {
+    x[0] = from_float<T>(a);
+    x[1] = from_float<T>(b);
+}
+template <> __device__ __forceinline__ void put2<__half>(__half* x, float a, float b) { *reinterpret_cast<__half2*>(x) = __floats2half2_rn(a, b); }
+template <> __device__ __forceinline__ void put2<__nv_bfloat16>(__nv_bfloat16* x, float a, float b) {
+    *reinterpret_cast<__nv_bfloat162*>(x) = __floats2bfloat162_rn(a, b);
+}
+
+// The VEC pairs of a unit, turned in place.
+template <typename T, int VEC, bool INTERLEAVED>
+__device__ __forceinline__ void turn_unit(Pack<T, VEC>& x0, Pack<T, VEC>& x1, const float2* cs) {
+    if constexpr (VEC == 1) {
+        const float f0 = to_float(x0.v[0]), f1 = to_float(x1.v[0]);
+        x0.v[0] = from_float<T>(f0 * cs[0].x - f1 * cs[0].y);
+        x1.v[0] = from_float<T>(f1 * cs[0].x + f0 * cs[0].y);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 2) {
+            const float4 two = *reinterpret_cast<const float4*>(cs + i);  // pairs i and i + 1; i even, so 16-byte aligned
+            if constexpr (INTERLEAVED) {
+                T* a = i < VEC / 2 ? &x0.v[2 * i] : &x1.v[2 * i - VEC];
+                T* b = i + 1 < VEC / 2 ? &x0.v[2 * i + 2] : &x1.v[2 * i + 2 - VEC];
+                const float2 f = get2(a), g = get2(b);
+                put2(a, f.x * two.x - f.y * two.y, f.y * two.x + f.x * two.y);
+                put2(b, g.x * two.z - g.y * two.w, g.y * two.z + g.x * two.w);
+            } else {
+                const float2 f = get2(&x0.v[i]), g = get2(&x1.v[i]);
+                put2(&x0.v[i], f.x * two.x - g.x * two.y, f.y * two.z - g.y * two.w);
+                put2(&x1.v[i], g.x * two.x + f.x * two.y, g.y * two.z + f.y * two.w);
+            }
+        }
+    }
+}
+
+template <typename T, int VEC, bool INTERLEAVED, int UNITS>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(RopeTensor q, RopeTensor k, RopeTensor v, RopeArgs a) {
     using P = Pack<T, VEC>;
-    extern __shared__ float2 turn_s[];  // cosine and sine of each pair, times mscale
+    extern __shared__ __align__(16) float2 turn_s[];  // cosine and sine of each pair, times mscale
     __shared__ int64_t place_s[2];      // page (-1: nothing is written) and place of the token
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
     const int half = int(a.rotary / 2), D = int(a.D), turned = half / VEC, threads = int(blockDim.x);
     const int per_head = turned + (D - int(a.rotary) + 2 * VEC - 1) / (2 * VEC);
-    const int units = (q.heads + k.heads + v.heads) * per_head, pass = threads * kRopeUnits;
+    const int units = (q.heads + k.heads + v.heads) * per_head, pass = threads * UNITS;
     for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
         bool ready = false;
         for (int base = int(blockIdx.y) * pass; base < units; base += pass * int(gridDim.y)) {
-            P x0[kRopeUnits], x1[kRopeUnits];
-            int which[kRopeUnits], unit[kRopeUnits], d0[kRopeUnits], d1[kRopeUnits];
-            int64_t out_at[kRopeUnits];
+            P x0[UNITS], x1[UNITS];
+            int which[UNITS], unit[UNITS], d0[UNITS], d1[UNITS];
+            int64_t out_at[UNITS];
 #pragma unroll
-            for (int j = 0; j < kRopeUnits; j++) {
+            for (int j = 0; j < UNITS; j++) {
                 const int w = base + j * threads + int(threadIdx.x);
                 which[j] = -1;
                 if (w >= units) continue;
@@ -63,8 +101,8 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(RopeTensor q, RopeTe
                     d0[j] = int(a.rotary) + (u - turned) * 2 * VEC;
                     d1[j] = d0[j] + VEC;
                 } else {
-                    d0[j] = a.interleaved ? u * 2 * VEC : u * VEC;
-                    d1[j] = a.interleaved ? d0[j] + VEC : d0[j] + half;
+                    d0[j] = INTERLEAVED ? u * 2 * VEC : u * VEC;
+                    d1[j] = INTERLEAVED ? d0[j] + VEC : d0[j] + half;
                 }
                 const T* in = static_cast<const T*>(is_q ? q.in : is_v ? v.in : k.in) +
                               t * (is_q ? q.in_t : is_v ? v.in_t : k.in_t) + h * (is_q ? q.in_h : is_v ? v.in_h : k.in_h);
@@ -93,7 +131,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(RopeTensor q, RopeTe
                 __syncthreads();
             }
 #pragma unroll
-            for (int j = 0; j < kRopeUnits; j++) {
+            for (int j = 0; j < UNITS; j++) {
                 if (which[j] < 0) continue;
                 T* out;
                 if (which[j] == 0) {
@@ -104,27 +142,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(RopeTensor q, RopeTe
                     out = static_cast<T*>(is_v ? v.out : k.out) + place_s[0] * (is_v ? v.out_t : k.out_t) +
                           place_s[1] * (is_v ? v.out_s : k.out_s) + out_at[j];
                 }
-                if (unit[j] < turned && which[j] != 2) {
-                    T e[2 * VEC];
-#pragma unroll
-                    for (int i = 0; i < VEC; i++) {
-                        e[i] = x0[j].v[i];
-                        e[VEC + i] = x1[j].v[i];
-                    }
-#pragma unroll
-                    for (int i = 0; i < VEC; i++) {
-                        const float2 cs = turn_s[unit[j] * VEC + i];
-                        const float f0 = to_float(a.interleaved ? e[2 * i] : e[i]), f1 = to_float(a.interleaved ? e[2 * i + 1] : e[VEC + i]);
-                        const T y0 = from_float<T>(f0 * cs.x - f1 * cs.y), y1 = from_float<T>(f1 * cs.x + f0 * cs.y);
-                        if (a.interleaved) {
-                            (2 * i < VEC ? x0[j].v[2 * i < VEC ? 2 * i : 0] : x1[j].v[2 * i < VEC ? 0 : 2 * i - VEC]) = y0;
-                            (2 * i + 1 < VEC ? x0[j].v[2 * i + 1 < VEC ? 2 * i + 1 : 0] : x1[j].v[2 * i + 1 < VEC ? 0 : 2 * i + 1 - VEC]) = y1;
-                        } else {
-                            x0[j].v[i] = y0;
-                            x1[j].v[i] = y1;
-                        }
-                    }
-                }
+                if (unit[j] < turned && which[j] != 2) turn_unit<T, VEC, INTERLEAVED>(x0[j], x1[j], turn_s + unit[j] * VEC);
                 *reinterpret_cast<P*>(out + d0[j]) = x0[j];
                 if (VEC > 1 || d1[j] < D) *reinterpret_cast<P*>(out + d1[j]) = x1[j];
             }
@@ -133,21 +151,26 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(RopeTensor q, RopeTe
     }
 }
 
+template <typename T, int VEC, int UNITS>
+int launch_rope_units(Ctx* ctx, const RopeTensor& q, const RopeTensor& k, const RopeTensor& v, const RopeArgs& a, int64_t units, bool share) {
+    int64_t threads = ceil_div(ceil_div(units, UNITS), 32) * 32;
+    if (threads > kRopeThreads) threads = kRopeThreads;
+    const int64_t y = share ? ceil_div(units, threads * UNITS) : 1;
+    const int64_t cap = int64_t(1) << 20;  // tokens beyond it are taken in turn
+    const size_t smem = size_t(a.rotary / 2) * sizeof(float2);
+    DOCC_CUDA_TRY(launch_pdl(a.interleaved ? rope_kernel<T, VEC, true, UNITS> : rope_kernel<T, VEC, false, UNITS>,
+                             dim3(unsigned(a.tokens < cap ? a.tokens : cap), unsigned(y)), dim3(unsigned(threads)), smem, ctx->stream, q, k, v, a));
+    return after_launch(ctx, "rope_kernel");
+}
 template <typename T, int VEC>
 int launch_rope(Ctx* ctx, const RopeTensor& q, const RopeTensor& k, const RopeTensor& v, const RopeArgs& a) {
     const int64_t per_head = a.rotary / 2 / VEC + ceil_div(a.D - a.rotary, 2 * VEC);
     const int64_t units = (int64_t(q.heads) + k.heads + v.heads) * per_head;
-    // few tokens: enough blocks per token that a thread has one round of units; many: a block per token, so that its angles are worked
-    // out once (8192 tokens of 384 units: 75 us with three blocks per token, 37 with one)
-    int64_t threads = ceil_div(ceil_div(units, kRopeUnits), 32) * 32;
-    if (threads > kRopeThreads) threads = kRopeThreads;
-    const int64_t shares = ceil_div(units, threads * kRopeUnits);
-    const int64_t y = a.tokens * shares <= 2 * int64_t(ctx->sm_count) ? shares : 1;
-    const int64_t cap = int64_t(1) << 20;
-    const size_t smem = size_t(a.rotary / 2) * sizeof(float2);
-    DOCC_CUDA_TRY(launch_pdl(rope_kernel<T, VEC>, dim3(unsigned(a.tokens < cap ? a.tokens : cap), unsigned(y)), dim3(unsigned(threads)), smem,
-                             ctx->stream, q, k, v, a));
-    return after_launch(ctx, "rope_kernel");
+    // Few tokens: a unit per thread, and as many blocks per token as that takes (16 tokens of 384 units: 2.1 us, with three units per
+    // thread 2.8). Many: a block per token and three units per thread, so that the angles are worked out once and 96 bytes per thread
+    // are on their way meanwhile (8192 tokens: 34.7 us; with two units 39, with one 41).
+    if (a.tokens * ceil_div(units, kRopeThreads) <= 2 * int64_t(ctx->sm_count)) return launch_rope_units<T, VEC, 1>(ctx, q, k, v, a, units, true);
+    return launch_rope_units<T, VEC, 3>(ctx, q, k, v, a, units, false);
 }
 
 template <typename T>
