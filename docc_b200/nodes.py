@@ -42,6 +42,12 @@ CODE_ATTENTION = "ml::Attention"  # no docc counterpart
 CODE_LAYERNORM = "ml::LayerNorm"  # no docc counterpart
 CODE_LINEAR = "ml::Linear"  # GEMM fused with its element-wise consumers; no docc counterpart
 CODE_CAST = "ml::Cast"
+# one decoding step; no docc counterparts
+CODE_RMSNORM = "ml::RMSNorm"
+CODE_ROPE = "ml::RoPE"
+CODE_ROPE_APPEND = "ml::RoPEAppend"
+CODE_PAGED_ATTENTION = "ml::PagedAttention"
+CODE_TOKEN_LOGPROBS = "ml::TokenLogProbs"
 
 
 class InvalidSDFGException(ValueError):
@@ -268,13 +274,91 @@ class LayerNormNode(LibraryNode):
         return {"eps": self.eps, "has_affine": self.has_affine}
 
 
+@dataclass
+class RMSNormNode(LibraryNode):
+    """Y = RMSNorm(X + R) * G, S = X + R (with a residual R). ``quantise`` replaces Y by the e4m3 codes Q and their scales: one per
+    ``group`` of 128 columns, or per row with group 0."""
+
+    eps: float = 1e-6
+    has_gamma: bool = True
+    has_residual: bool = False
+    quantise: bool = False
+    group: int = 0
+    code: str = CODE_RMSNORM
+    input_connectors: Sequence[str] = ("X", "G", "R")
+
+    def __post_init__(self):
+        self.output_connectors = (("Q", "C") if self.quantise else ("Y",)) + (("S",) if self.has_residual else ())
+
+    def _params(self) -> dict:
+        return {"eps": self.eps, "has_gamma": self.has_gamma, "has_residual": self.has_residual, "quantise": self.quantise, "group": self.group}
+
+
+@dataclass
+class RoPENode(LibraryNode):
+    """Rotary positions on X [tokens, heads, D]; ``inverse`` is the transpose (and gradient) of the map."""
+
+    interleaved: bool = False
+    mscale: float = 1.0
+    inverse: bool = False
+    code: str = CODE_ROPE
+    input_connectors: Sequence[str] = ("X", "P", "F")
+    output_connectors: Sequence[str] = ("Y",)
+
+    def _params(self) -> dict:
+        return {"interleaved": self.interleaved, "mscale": self.mscale, "inverse": self.inverse}
+
+
+@dataclass
+class RoPEAppendNode(LibraryNode):
+    """Rotates Q and K and writes K and V into the paged cache KC, VC at the slots L; the caches are updated in place."""
+
+    interleaved: bool = False
+    mscale: float = 1.0
+    code: str = CODE_ROPE_APPEND
+    input_connectors: Sequence[str] = ("Q", "K", "V", "P", "F", "KC", "VC", "L")
+    output_connectors: Sequence[str] = ("Y",)
+
+    def _params(self) -> dict:
+        return {"interleaved": self.interleaved, "mscale": self.mscale}
+
+
+@dataclass
+class PagedAttentionNode(LibraryNode):
+    """Attention of one new token per sequence over the paged cache KC, VC with page table T and lengths N."""
+
+    scale: Optional[float] = None
+    softcap: float = 0.0
+    window: int = 0
+    code: str = CODE_PAGED_ATTENTION
+    input_connectors: Sequence[str] = ("Q", "KC", "VC", "T", "N")
+    output_connectors: Sequence[str] = ("O",)
+
+    def _params(self) -> dict:
+        return {"scale": self.scale, "softcap": self.softcap, "window": self.window}
+
+
+@dataclass
+class TokenLogProbsNode(LibraryNode):
+    """Log-probabilities L of the tokens I under softmax(scale * X), entropies H, and the k likeliest tokens TI with theirs, TL."""
+
+    k: int = 0
+    scale: float = 1.0
+    code: str = CODE_TOKEN_LOGPROBS
+    input_connectors: Sequence[str] = ("X", "I")
+    output_connectors: Sequence[str] = ("L", "H", "TI", "TL")
+
+    def _params(self) -> dict:
+        return {"k": self.k, "scale": self.scale}
+
+
 # ---- target mapping -------------------------------------------------------------------------------
 class B200LibraryNodeMapper:
     """Picks the implementation type for nodes the B200 runtime executes. Everything it does not
     recognise is left untouched (and will fail at dispatch: there is no expansion to loop nests)."""
 
     MAPPED = {CODE_GEMM, CODE_MATMUL, CODE_SOFTMAX, CODE_CONV, CODE_ELEMENTWISE, CODE_ATTENTION, CODE_LAYERNORM, CODE_LINEAR,
-              CODE_CAST, *CODE_REDUCE.values()}
+              CODE_CAST, CODE_RMSNORM, CODE_ROPE, CODE_ROPE_APPEND, CODE_PAGED_ATTENTION, CODE_TOKEN_LOGPROBS, *CODE_REDUCE.values()}
 
     def __init__(self, with_transfers: bool = True):
         self.impl = IMPL_B200_WITH_TRANSFERS if with_transfers else IMPL_B200_WITHOUT_TRANSFERS
@@ -407,11 +491,37 @@ def _layernorm(node: LayerNormNode, env: dict) -> None:
     env[node.outputs[0]] = ops.layernorm(x, g, b, node.eps)
 
 
+def _rmsnorm(node: RMSNormNode, env: dict) -> None:
+    x = env[node.inputs[0]]
+    g = env[node.inputs[1]] if node.has_gamma else None
+    r = env[node.inputs[2]] if node.has_residual else None
+    y = ops.rmsnorm_quant(x, g, r, node.eps, node.group) if node.quantise else ops.rmsnorm(x, g, r, node.eps)
+    env.update(zip(node.outputs, y if isinstance(y, tuple) else (y,)))
+
+
+def _rope(node: RoPENode, env: dict) -> None:
+    x, p, f = (env[n] for n in node.inputs[:3])
+    env[node.outputs[0]] = ops.rope(x, p, f, node.interleaved, node.mscale, node.inverse)
+
+
+def _rope_append(node: RoPEAppendNode, env: dict) -> None:
+    env[node.outputs[0]] = ops.rope_append(*(env[n] for n in node.inputs[:8]), interleaved=node.interleaved, mscale=node.mscale)
+
+
+def _paged_attention(node: PagedAttentionNode, env: dict) -> None:
+    env[node.outputs[0]] = ops.paged_attention(*(env[n] for n in node.inputs[:5]), scale=node.scale, softcap=node.softcap, window=node.window)
+
+
+def _token_logprobs(node: TokenLogProbsNode, env: dict) -> None:
+    env.update(zip(node.outputs, ops.token_logprobs(env[node.inputs[0]], env[node.inputs[1]], node.k, node.scale)))
+
+
 def register_b200_plugin(registry: LibraryNodeDispatcherRegistry) -> None:
     """The ``register_plugin(plugins::Context&)`` of a docc target (targets/et/src/et/target.cpp:21-36)."""
     table = {CODE_GEMM: _gemm, CODE_MATMUL: _matmul, CODE_SOFTMAX: _softmax, CODE_CONV: _conv,
              CODE_ELEMENTWISE: _elementwise, CODE_CAST: _cast, CODE_LINEAR: _linear, CODE_ATTENTION: _attention,
-             CODE_LAYERNORM: _layernorm}
+             CODE_LAYERNORM: _layernorm, CODE_RMSNORM: _rmsnorm, CODE_ROPE: _rope, CODE_ROPE_APPEND: _rope_append,
+             CODE_PAGED_ATTENTION: _paged_attention, CODE_TOKEN_LOGPROBS: _token_logprobs}
     for code in CODE_REDUCE.values():
         table[code] = _reduce
     for code, fn in table.items():

@@ -155,6 +155,15 @@ def _layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
     return _dispatch(node, _contig(x), _f32(weight), _f32(bias))
 
 
+def _rms_norm(x, normalized_shape, weight=None, eps=None):
+    if len(tuple(normalized_shape)) != 1:
+        raise UnsupportedGraph("rms_norm over more than the last dimension")
+    if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise UnsupportedGraph(f"rms_norm of {x.dtype}")
+    eps = torch.finfo(torch.float32).eps if eps is None else eps  # torch's default: that of the type it computes in
+    return _dispatch(N.RMSNormNode(eps=eps, has_gamma=weight is not None), _contig(x), _contig(_f32(weight)) if weight is not None else None)
+
+
 def _unary(kind):
     def fn(x, *args, **kwargs):
         if kind == "gelu" and kwargs.get("approximate", "none") != "none":
@@ -204,7 +213,7 @@ _FUNCTIONS: Dict[object, Callable] = {
     F.softmax: _softmax, torch.softmax: _softmax,
     F.conv2d: _conv2d, torch.conv2d: _conv2d,
     F.scaled_dot_product_attention: _sdpa, torch._C._nn.scaled_dot_product_attention: _sdpa,
-    F.layer_norm: _layer_norm,
+    F.layer_norm: _layer_norm, F.rms_norm: _rms_norm, torch.rms_norm: _rms_norm,
     F.gelu: _unary("gelu"), torch._C._nn.gelu: _unary("gelu"), F.relu: _unary("relu"), torch.relu: _unary("relu"),
     torch.tanh: _unary("tanh"), F.tanh: _unary("tanh"), torch.sigmoid: _unary("sigmoid"), F.sigmoid: _unary("sigmoid"),
     torch.exp: _unary("exp"), torch.erf: _unary("erf"), torch.sqrt: _unary("sqrt"), torch.abs: _unary("abs"),
