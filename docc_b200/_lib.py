@@ -108,5 +108,13 @@ def check(status: int, name: str) -> None:
         raise DoccB200Error(status, name, detail)
 
 
+_functions = {}  # name -> bound function
+
+
 def call(name: str, *args) -> None:
-    check(getattr(lib(), name)(*args), name)
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(lib(), name)
+    status = fn(*args)
+    if status != 0:
+        check(status, name)

@@ -359,6 +359,16 @@ def layernorm(X, gamma=None, beta=None, eps=1e-5, flags=0):
 # These calls are short on the device, so that what the host does around them is most of a step: the helpers ask a tensor for as
 # little as the checks need.
 _Pairs, _Triples = _i64 * 2, _i64 * 3
+_torch = None  # the module, once one of its tensors has been met (an import statement costs as much as several of the checks)
+
+
+def _torch_module():
+    global _torch
+    if _torch is None:
+        import torch
+
+        _torch = torch
+    return _torch
 
 
 def _addr(x):
@@ -385,9 +395,7 @@ def _side(*xs):
                 if at < 0:
                     raise TypeError("torch tensors must live on a CUDA device (pass numpy arrays for host data)")
                 if current is None:
-                    import torch
-
-                    current = torch.cuda.current_device()
+                    current = (_torch or _torch_module()).cuda.current_device()
                 if at != current:
                     raise ValueError(f"tensor on cuda:{at} while the calling thread's device is cuda:{current}")
             device = True
@@ -405,9 +413,7 @@ def _side(*xs):
 def _new_like(x):
     """An uninitialised contiguous array of x's kind, shape and element type."""
     if _is_torch(x) and x.is_contiguous():
-        import torch
-
-        return torch.empty_like(x)
+        return (_torch or _torch_module()).empty_like(x)
     return _new(x, x.shape)
 
 
@@ -472,11 +478,10 @@ _torch_dtypes = {}
 def _like(x, name):
     """The element type ``name`` in the library ``x`` comes from."""
     if _is_torch(x):
-        if name not in _torch_dtypes:
-            import torch
-
-            _torch_dtypes[name] = getattr(torch, name)
-        return _torch_dtypes[name]
+        got = _torch_dtypes.get(name)
+        if got is None:
+            got = _torch_dtypes[name] = getattr(_torch_module(), name)
+        return got
     return np.dtype(name)
 
 
@@ -615,12 +620,6 @@ def rope_append(q, k, v, positions, inv_freq, k_cache, v_cache, slots, interleav
     return out
 
 
-def _capturing():
-    import torch
-
-    return torch.cuda.is_current_stream_capturing()
-
-
 _scratch_bytes = {}  # (device, query heads per key-value head, D) -> bytes: what the size of the scratch depends on
 
 
@@ -650,7 +649,7 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, scale=None, softca
     out = _out_like(q, out, "paged_attention")
     lse = _new(q, (B, Hq), "float32") if return_lse else None
     work, bytes_ = None, 0
-    if _is_torch(q) and _capturing():
+    if _is_torch(q) and _torch_module().cuda.is_current_stream_capturing():
         key = (q.get_device(), Hq // Hkv, D)
         bytes_ = _scratch_bytes.get(key)
         if bytes_ is None:
@@ -673,7 +672,10 @@ def token_logprobs(logits, ids, k=0, scale=1.0, flags=0):
         raise ValueError("token_logprobs: logits must be [rows, vocab]")
     rows, vocab, ldx = _rows_of(logits, "token_logprobs")
     _want(ids, "int64", "token_logprobs: ids", (rows,))
-    logp, entropy = _new(logits, (rows,), "float32"), _new(logits, (rows,), "float32")
+    if _is_torch(logits):
+        logp, entropy = _new(logits, (2, rows), "float32").unbind(0)
+    else:
+        logp, entropy = _new(logits, (rows,), "float32"), _new(logits, (rows,), "float32")
     top_ids, top_logp = _new(ids, (rows, k)), _new(logits, (rows, k), "float32")
     call("docc_b200_token_logprobs", _prec(logits), rows, vocab, _addr(logits), ldx, scale, _addr(ids), _addr(logp), _addr(entropy), k,
          _addr(top_ids), _addr(top_logp), flags)
