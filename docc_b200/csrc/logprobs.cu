@@ -263,9 +263,10 @@ struct Scan {
 __device__ __forceinline__ uint32_t ordered(float x) { return uint32_t(rank_key(x, 0) >> 32); }
 
 // A value (as ordered bits) that at least k of the block's threads reach with theirs, near the k-th largest: a warp's j-th largest,
-// j = ceil(k / warps), of the r-th best warp, j r >= k. `values_s` has room for one word per warp. 0 if there is none.
-template <int WARPS> __device__ __forceinline__ uint32_t bound_of(uint32_t mine, int k, uint32_t* values_s, int lane, int warp) {
-    const int j = (k + WARPS - 1) / WARPS, r = (k + j - 1) / j;
+// j = ceil(k / active), of the r-th best warp, j r >= k. active: the warps whose every lane has values. `values_s` has room for one word
+// per warp. 0 if there is none.
+template <int WARPS> __device__ __forceinline__ uint32_t bound_of(uint32_t mine, int k, int active, uint32_t* values_s, int lane, int warp) {
+    const int j = (k + active - 1) / active, r = (k + j - 1) / j;
     uint32_t rest = mine, nth = 0;
     for (int i = 0; i < j; i++) {
         nth = __reduce_max_sync(0xffffffffu, rest);
@@ -297,8 +298,6 @@ __device__ __forceinline__ void rank_keys(const uint64_t* keys, int n, int k, ui
     }
 }
 
-// BLOCK: 256 threads without alternatives, where nothing but the stream counts (141 us for 4096 rows of 50021 fp32, with 512: 153); 512
-// with them, since what follows the stream takes a block's time whatever its size (256 rows of 128000: 20.3 us, with 256: 25.8).
 template <typename T, bool TOP, int BLOCK>
 __global__ void __launch_bounds__(BLOCK, 1024 / BLOCK) logprobs_kernel(const T* __restrict__ X, LogpArgs a, int log_ranks) {
     constexpr int VEC = 16 / sizeof(T), UNROLL = 4, WARPS = BLOCK / 32;
@@ -351,7 +350,7 @@ __global__ void __launch_bounds__(BLOCK, 1024 / BLOCK) logprobs_kernel(const T* 
         if constexpr (TOP) {
             if (t == 0) n_streams = n_found = n_hits = 0;
             if (scan.best > -INFINITY) key = ordered(scan.best);
-            bar = uint64_t(bound_of<WARPS>(key, a.k, values_s, lane, warp)) << 32;  // 0: too few threads have a logit above -inf, all is looked at
+            bar = uint64_t(bound_of<WARPS>(key, a.k, max(1, min(WARPS, (p1 - p0) / 32)), values_s, lane, warp)) << 32;  // 0: too few threads have a logit above -inf, all is looked at
         } else {
             __syncthreads();
         }
@@ -466,9 +465,8 @@ __global__ void __launch_bounds__(BLOCK, 1024 / BLOCK) logprobs_kernel(const T* 
     }
 }
 
-template <typename T, bool TOP>
+template <typename T, bool TOP, int BLOCK>
 int launch_logprobs(Ctx* ctx, const void* X, const LogpArgs& a) {
-    constexpr int BLOCK = TOP ? 512 : 256;
     // clusters only while every block has an SM of its own: at 256 rows two blocks per row took 29 us instead of 20, eight took 53
     int ranks = 1, log_ranks = 0;
     while (ranks < 8 && a.rows * ranks * 2 <= ctx->sm_count && a.vocab / (2 * ranks) >= 2048) {
@@ -494,7 +492,13 @@ int launch_logprobs(Ctx* ctx, const void* X, const LogpArgs& a) {
 }
 template <typename T>
 int logprobs_device(Ctx* ctx, const void* X, const LogpArgs& a) {
-    return a.k ? launch_logprobs<T, true>(ctx, X, a) : launch_logprobs<T, false>(ctx, X, a);
+    // What follows the stream takes a block's time whatever the row's length, so short rows want small blocks, many to an SM, and long
+    // ones large blocks. bf16, k = 20: 2000 rows of 32768 51 us with 128 threads, 54 with 256, 66 with 512; 600 of 128000 77, 60 and 52;
+    // 64 of 20000, fewer than fill the SMs, 10.5, 8.8 and 8.4. k = 0: 1000 of 9000 5.9 with 128, 7.6 with 256; 600 of 60000 22.5 and 17.
+    const bool is_short = a.vocab * int64_t(sizeof(T)) <= 64 * 1024, many = a.rows > 2 * int64_t(ctx->sm_count);
+    if (is_short && many) return a.k ? launch_logprobs<T, true, 128>(ctx, X, a) : launch_logprobs<T, false, 128>(ctx, X, a);
+    if (is_short || !a.k) return a.k ? launch_logprobs<T, true, 256>(ctx, X, a) : launch_logprobs<T, false, 256>(ctx, X, a);
+    return launch_logprobs<T, true, 512>(ctx, X, a);
 }
 
 int logprobs_any(Ctx* ctx, int prec, const void* X, const LogpArgs& a) {
