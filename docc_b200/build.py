@@ -3,14 +3,20 @@
 ``python -m docc_b200.build`` compiles every ``csrc/*.cu`` into an object file (in
 parallel) and links them into ``docc_b200/lib/libdocc_b200_rt.so``. The library has
 no Python or torch dependency; the CUDA runtime is linked statically.
+
+Where torch is installed, ``host/decode_calls.cpp`` is compiled beside it: the host side of
+the shortest calls of ``docc_b200.ops`` for torch tensors, which reaches the library through
+the addresses that ``ops`` binds and is not linked with it.
 """
 from __future__ import annotations
 
 import hashlib
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
@@ -19,6 +25,8 @@ CSRC = os.path.join(_PKG, "csrc")
 INCLUDE = os.path.join(_ROOT, "include")
 LIB_DIR = os.path.join(_PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libdocc_b200_rt.so")
+HOST_SRC = os.path.join(_PKG, "host", "decode_calls.cpp")
+HOST_PATH = os.path.join(LIB_DIR, "docc_b200_decode_calls.so")
 _OBJ_DIR = os.path.join(_PKG, "build", "obj")
 _STAMP = os.path.join(LIB_DIR, "libdocc_b200_rt.stamp")
 
@@ -45,6 +53,7 @@ def source_hash() -> str:
     h = hashlib.sha256()
     files = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith((".cu", ".cuh", ".h"))]
     files.append(os.path.join(INCLUDE, "docc_b200", "rt.h"))
+    files.append(HOST_SRC)
     for path in files:
         h.update(os.path.basename(path).encode())
         with open(path, "rb") as fh:
@@ -54,10 +63,29 @@ def source_hash() -> str:
 
 
 def is_current() -> bool:
-    if not (os.path.exists(LIB_PATH) and os.path.exists(_STAMP)):
+    if not (os.path.exists(LIB_PATH) and os.path.exists(_STAMP)) or (_torch_root() and not os.path.exists(HOST_PATH)):
         return False
     with open(_STAMP) as fh:
         return fh.read().strip() == source_hash()
+
+
+def _torch_root():
+    """The installed torch package's folder, without importing it; None if there is none."""
+    spec = importlib.util.find_spec("torch")
+    return spec.submodule_search_locations[0] if spec and spec.submodule_search_locations else None
+
+
+def _build_host() -> None:
+    torch = _torch_root()
+    if torch is None:
+        return
+    cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-I" + INCLUDE,
+           "-I" + os.path.join(torch, "include"), "-I" + os.path.join(torch, "include", "torch", "csrc", "api", "include"),
+           "-I" + sysconfig.get_paths()["include"], HOST_SRC, "-o", HOST_PATH, "-L" + os.path.join(torch, "lib"), "-lc10", "-ltorch_cpu",
+           "-ltorch_python", "-ltorch"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on {os.path.basename(HOST_SRC)}:\n{res.stdout}\n{res.stderr}")
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -86,6 +114,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     res = subprocess.run(link, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
+    _build_host()
     with open(_STAMP, "w") as fh:
         fh.write(source_hash())
     return LIB_PATH

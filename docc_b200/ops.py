@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import os
 
 import numpy as np
 
@@ -381,6 +382,33 @@ def _addr(x):
         return x.ctypes.data
 
 
+_NATIVE = ("docc_b200_rmsnorm", "docc_b200_rmsnorm_q8", "docc_b200_rope", "docc_b200_rope_append", "docc_b200_paged_attention",
+           "docc_b200_token_logprobs")
+_native = None  # the compiled form of these calls for torch tensors (docc_b200/host); None until the first of them
+
+
+def _compiled(x):
+    """The module that takes the ordinary call on torch tensors; it answers None to every other, which then runs here. False before the
+    first torch tensor has been met."""
+    global _native
+    if _native is None:
+        if not _is_torch(x):
+            return False
+        from importlib.machinery import ExtensionFileLoader
+        from importlib.util import module_from_spec, spec_from_loader
+
+        from .build import HOST_PATH
+
+        if not os.path.exists(HOST_PATH):
+            raise RuntimeError(f"{HOST_PATH} is missing: run `python -m docc_b200.build`.")
+        loader = ExtensionFileLoader("docc_b200_decode_calls", HOST_PATH)
+        module = module_from_spec(spec_from_loader(loader.name, loader))
+        loader.exec_module(module)
+        module.bind(*(ctypes.cast(getattr(_lib.lib(), name), _vp).value for name in _NATIVE))
+        _native = module
+    return _native
+
+
 def _side(*xs):
     """``_kind`` without its demand for contiguity, for entries that take strides: flags, after checking that all arrays live on the
     same side and, for torch tensors, on the device that the calling thread's launches go to."""
@@ -503,6 +531,11 @@ def _rms_inputs(X, gamma, residual, flags):
 def rmsnorm(X, gamma=None, residual=None, eps=1e-6, flags=0):
     """``Y = s / sqrt(mean(s^2) + eps) * gamma`` over the last dimension, ``s = X + residual``. Returns Y, or with a residual
     ``(Y, S)``: S is s in the input's type, the residual of what follows. ``gamma`` is float32."""
+    native = _native or _compiled(X)
+    if native and not flags:
+        got = native.rmsnorm(X, gamma, residual, eps)
+        if got is not None:
+            return got
     rows, cols, ldx, ldr, flags = _rms_inputs(X, gamma, residual, flags)
     Y = _new_like(X)
     S = _new_like(X) if residual is not None else None
@@ -514,6 +547,11 @@ def rmsnorm_quant(X, gamma=None, residual=None, eps=1e-6, group=0, flags=0):
     """The norm of ``rmsnorm`` with an 8-bit output: ``(Q, scales)``, or ``(Q, scales, S)`` with a residual. Q holds e4m3 values
     (``torch.float8_e4m3fn``; their codes as uint8 for other arrays) and ``Q * scales`` stands for the norm, with one float32 scale
     per ``group`` of 128 columns or, with group 0, per row: scales have shape ``X.shape[:-1] + (groups,)``."""
+    native = _native or _compiled(X)
+    if native and not flags:
+        got = native.rmsnorm_quant(X, gamma, residual, eps, group)
+        if got is not None:
+            return got
     rows, cols, ldx, ldr, flags = _rms_inputs(X, gamma, residual, flags)
     if group not in (0, 128):
         raise ValueError("rmsnorm_quant: group must be 0 (whole rows) or 128")
@@ -576,6 +614,11 @@ def rope(X, positions, inv_freq, interleaved=False, mscale=1.0, inverse=False, o
     """Rotary positions on X [tokens, heads, D] (``docc_b200_rope``): ``positions`` int64 [tokens], ``inv_freq`` float64
     [rotary_dim / 2] on the side of X (``rope_frequencies``). ``inverse`` applies the transpose, which is the gradient. ``out`` may be
     X itself."""
+    native = _native or _compiled(X)
+    if native and not flags:
+        got = native.rope(X, positions, inv_freq, interleaved, mscale, inverse, out)
+        if got is not None:
+            return got
     flags |= _side(X, positions, inv_freq, out)
     if X.ndim != 3:
         raise ValueError("rope: X must be [tokens, heads, D]")
@@ -601,6 +644,11 @@ def rope_append(q, k, v, positions, inv_freq, k_cache, v_cache, slots, interleav
     """Rotates q [tokens, Hq, D] and k [tokens, Hkv, D] and writes the rotated k and v into the paged cache
     [pages, Hkv, page_size, D] at ``slots`` (int64 [tokens]: page * page_size + place; negative: not written). Returns the rotated q
     (``out``, which may be q itself). Device tensors only; the slots of one call must differ."""
+    native = _native or _compiled(q)
+    if native and not flags:
+        got = native.rope_append(q, k, v, positions, inv_freq, k_cache, v_cache, slots, interleaved, mscale, out)
+        if got is not None:
+            return got
     if _side(q, k, v, positions, inv_freq, k_cache, v_cache, slots, out):
         raise TypeError("rope_append: the cache lives on the device; host arrays are not taken")
     if q.ndim != 3 or k.ndim != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
@@ -632,6 +680,11 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, scale=None, softca
 
     While torch captures a graph the scratch comes from torch's allocator, so that the graph owns what it replays with; otherwise it
     is the library's, ordered on the calling thread's stream."""
+    native = _native or _compiled(q)
+    if native and not flags:
+        got = native.paged_attention(q, k_cache, v_cache, page_table, lengths, scale, softcap, window, return_lse, out)
+        if got is not None:
+            return got
     if _side(q, k_cache, v_cache, page_table, lengths, out):
         raise TypeError("paged_attention: the cache lives on the device; host arrays are not taken")
     if q.ndim != 3 or k_cache.ndim != 4:
@@ -667,6 +720,11 @@ def token_logprobs(logits, ids, k=0, scale=1.0, flags=0):
     """``(logp, entropy, top_ids, top_logp)`` of logits [rows, vocab] under ``softmax(scale * logits)``: the log-probability of token
     ``ids[row]`` (int64; an id outside the vocabulary gives NaN), the distribution's entropy, and the ``k`` <= 32 most likely tokens
     with their log-probabilities (ties to the lowest index). float32, indices int64; [rows, k] for the last two."""
+    native = _native or _compiled(logits)
+    if native and not flags:
+        got = native.token_logprobs(logits, ids, k, scale)
+        if got is not None:
+            return got
     flags |= _side(logits, ids)
     if logits.ndim != 2:
         raise ValueError("token_logprobs: logits must be [rows, vocab]")
