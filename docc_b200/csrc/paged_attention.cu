@@ -939,7 +939,7 @@ extern "C" int docc_b200_paged_attention(int prec, int64_t B, int64_t Hq, int64_
                  "paged_attention: precision %d not supported (use 's', 'b' or 'h')", prec);
     DOCC_REQUIRE(B >= 0 && Hq >= 0 && Hkv >= 0 && D >= 0 && num_pages >= 0 && max_pages >= 0, "paged_attention: negative extent");
     DOCC_REQUIRE(page_size > 0, "paged_attention: page_size must be positive");
-    DOCC_REQUIRE(softcap >= 0.f && window >= 0, "paged_attention: softcap and window must not be negative");
+    DOCC_REQUIRE(softcap >= 0.f && softcap < INFINITY && window >= 0, "paged_attention: softcap must be finite, and neither it nor window negative");
     if (flags & DOCC_B200_FLAG_HOST_PTRS)
         return set_error(DOCC_B200_ERR_UNSUPPORTED, "paged_attention: the cache lives on the device; host pointers are not taken");
     Ctx* ctx;

@@ -639,7 +639,7 @@ def test_refusals_of_the_c_abi():
     attend = lambda prec=S, page=4, cap=0.0, window=0, flags=0: status_of(
         "docc_b200_paged_attention", prec, 1, 1, 1, 8, 1.0, cap, window, 16, None, 16, None, 16, None, 1, page, 16, 1, 1, 16, 16, None, None, None, 0, flags)
     assert attend(prec=ord("d")) == INVALID and attend(page=0) == INVALID and attend(cap=-1.0) == INVALID and attend(window=-1) == INVALID
-    assert attend(flags=1) == UNSUPPORTED
+    assert attend(flags=1) == UNSUPPORTED and attend(cap=float("inf")) == INVALID and attend(cap=float("nan")) == INVALID
     logp = lambda k=0, scale=1.0, prec=S: status_of("docc_b200_token_logprobs", prec, 1, 8, 16, 8, scale, 16, 16, 16, k, 16, 16, 0)
     assert logp(k=9) == INVALID and logp(k=33) == INVALID and logp(k=-1) == INVALID and logp(scale=0.0) == INVALID
     assert logp(scale=float("nan")) == INVALID and logp(prec=ord("d")) == INVALID

@@ -289,6 +289,71 @@ def test_a_chain_of_launches_sees_what_the_one_before_wrote(rt):
     assert torch.equal(a, b) and torch.equal(ra, rb)
 
 
+# ---- the compiled host side -----------------------------------------------------------------------------------------------------------
+def test_the_compiled_calls_answer_none_to_what_they_do_not_take():
+    module = ops._compiled(torch.zeros(1))
+    assert module and module is ops._native
+    x = torch.zeros(2, 3)
+    for name, count in (("rmsnorm", 4), ("rmsnorm_quant", 5), ("rope", 7), ("rope_append", 11), ("paged_attention", 10), ("token_logprobs", 4)):
+        fn = getattr(module, name)
+        assert fn() is None and fn(*[None] * count) is None and fn(*[x] * count) is None and fn(*["a"] * count) is None
+        assert fn(*[x.numpy()] * count) is None and fn(*[1.5] * (count + 3)) is None
+
+
+def both_ways(monkeypatch, call):
+    """The call through the compiled host side, with proof that it took it, and through the Python one."""
+    taken = []
+
+    class Spy:
+        def __getattr__(self, name):
+            def fn(*args):
+                got = getattr(module, name)(*args)
+                taken.append(got is not None)
+                return got
+
+            return fn
+
+    module = ops._compiled(torch.zeros(1))
+    monkeypatch.setattr(ops, "_native", Spy())
+    compiled = call()
+    settle()
+    monkeypatch.setattr(ops, "_native", None)
+    monkeypatch.setattr(ops, "_compiled", lambda x: False)
+    plain = call()
+    settle()
+    monkeypatch.undo()
+    assert taken == [True]
+    compiled, plain = (r if isinstance(r, tuple) else (r,) for r in (compiled, plain))
+    assert len(compiled) == len(plain)
+    for a, b in zip(compiled, plain):
+        assert a.dtype == b.dtype and a.shape == b.shape and a.stride() == b.stride() and a.device == b.device and not a.requires_grad
+        torch.testing.assert_close(a.float(), b.float(), rtol=0, atol=0, equal_nan=True)  # NaN: the id that is no token
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_both_host_sides_make_the_same_call(rt, monkeypatch, dtype):
+    wide = normal(6, 1000, seed=1, dtype=dtype).cuda()
+    x, r, g = wide[:, :256], wide[:, 256:512], torch.nn.Parameter(normal(256, seed=2).cuda())
+    both_ways(monkeypatch, lambda: ops.rmsnorm(x, g, r))
+    both_ways(monkeypatch, lambda: ops.rmsnorm(x.contiguous().view(2, 3, 256)))
+    both_ways(monkeypatch, lambda: ops.rmsnorm_quant(x, g, r, group=128))
+    both_ways(monkeypatch, lambda: ops.rmsnorm_quant(x.contiguous().view(2, 3, 256), group=0, eps=1e-5))
+    q, k, v = (t.unflatten(1, (-1, 32)) for t in wide[:, : 32 * 12].split([256, 64, 64], dim=1))
+    pos, freq = torch.arange(6).cuda(), torch.from_numpy(ops.rope_frequencies(32)[0]).cuda()
+    both_ways(monkeypatch, lambda: ops.rope(q, pos, freq, interleaved=True, mscale=2))
+    both_ways(monkeypatch, lambda: ops.rope(q, pos, freq, inverse=True, out=torch.empty(6, 16, 32, dtype=dtype, device="cuda")[:, ::2]))
+    slots = torch.tensor([3, 9, -1, 0, 15, 7]).cuda()
+    kc, vc = normal(4, 2, 4, 32, seed=5, dtype=dtype).cuda(), normal(4, 4, 2, 32, seed=6, dtype=dtype).cuda().transpose(1, 2)
+    both_ways(monkeypatch, lambda: (ops.rope_append(q, k, v, pos, freq, kc, vc, slots), kc.clone(), vc.contiguous()))
+    table, lengths = torch.arange(4).int().cuda().view(2, 2), torch.tensor([7, 5], dtype=torch.int32).cuda()
+    both_ways(monkeypatch, lambda: ops.paged_attention(q[:2], kc, vc, table, lengths, return_lse=True))
+    both_ways(monkeypatch, lambda: ops.paged_attention(q[:2].contiguous(), kc, vc, table, lengths, scale=0.3, softcap=4, window=3))
+    ids = torch.tensor([0, 5, 999, -1, 4, 2]).cuda()
+    both_ways(monkeypatch, lambda: ops.token_logprobs(wide, ids)[:2])
+    both_ways(monkeypatch, lambda: ops.token_logprobs(wide[:, :700], ids, k=4, scale=0.5))
+
+
 # ---- torch.compile ------------------------------------------------------------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("dtype,tol", [(torch.float32, 1e-4), (torch.bfloat16, 2e-2)])
