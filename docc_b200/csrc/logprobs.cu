@@ -10,6 +10,10 @@
 // bound of the row's k-th largest, and only those threads can hold others: some thirty of 512 for k = 20. Their logits are read again
 // (from L2), and what reaches T, few more than k values, is ranked by counting.
 //
+// 4096 rows of 50021 fp32 without alternatives: 820 MB, 138 us (5.9 TB/s, 0.91 of the measured copy); 256 rows of 128000 bf16 with
+// twenty: 22.5 us, about 11 for the stream and the rest for what follows it, which nothing overlaps while all rows run at once; 4 rows
+// of 32768: 5.9 us.
+//
 // With fewer rows than fill the machine, a cluster of up to eight blocks takes a row; the other blocks' sums and lists meet in the first
 // block through distributed shared memory, in the order of the ranks.
 #include "common.cuh"

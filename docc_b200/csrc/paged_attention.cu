@@ -14,6 +14,12 @@
 //     result on every call.
 //   * Inside a block every warp has its own keys of each chunk, its own ring of asynchronous copies and its own running maximum and
 //     sum: nothing synchronises but the merge of the four warps at the end of a row.
+//
+// Measured (bf16 / fp16, heads of 128, fresh inputs per call): 64 ragged sequences up to 8192 tokens, 32 heads on 8, 609 MB: 116 us
+// (5.2 TB/s, 0.80 of the measured copy); one of 131079 tokens, 16 heads on 2, capped scores, 134 MB: 36.5 us, of which the stream is 25,
+// the first chunk's way through lengths, page table and keys 3, the join 8 with its launch; one of 1025: 9.8 us. In an early form the
+// median block of the first case was done after 102 us and the slowest, with a run of short rows, after 142: hence kRowCost. More runs
+// than resident blocks gained nothing (147, 155 and 166 us with 2, 4 and 8 times as many).
 #include <atomic>
 #include <type_traits>
 

@@ -3,7 +3,8 @@
 //   s = x + r,  S = round(s),  y = s * rsqrt(mean(s^2) + eps) * gamma,  Y = round(y)  or  Q = e4m3(y / scale_g)
 //
 // Bandwidth bound: x and r are read once, S and Y (or Q and its scales) written once. s stays in fp32 between the sum of
-// squares and the output, so each output is rounded once.
+// squares and the output, so each output is rounded once. Rows of 8192 x 4096 bf16 with residual and 8-bit output: 236 MB, 44.7 us with
+// fresh outputs per call (5.3 TB/s, 0.81 of the measured copy), 38.6 us replayed on the same ones; 8 rows of 1024: 2.0 us.
 #include <cuda_fp8.h>
 
 #include "common.cuh"

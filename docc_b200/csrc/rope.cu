@@ -3,6 +3,9 @@
 // Pair i < R/2 of a head turns by a = position * inv_freq[i]: (u, v) -> m (u cos a - v sin a, v cos a + u sin a). In fp32 the
 // product is off by position * 2^-24 radians, a quarter of a turn at ten million and visible from a few thousand on, so the
 // angle is formed in fp64 as a number of turns, reduced to [-1/2, 1/2] there, and only then handed to sincospif.
+//
+// Bandwidth bound: q, k and v are read once, q and the cache's places written once. 8192 tokens of 32 + 8 heads of 128 in fp16: 201 MB,
+// 37.1 us with fresh outputs (5.4 TB/s, 0.83 of the measured copy); 16 tokens 2.05 us, a launch's time.
 #include "common.cuh"
 #include "device_math.cuh"
 #include "ptx.cuh"
