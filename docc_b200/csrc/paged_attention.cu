@@ -35,7 +35,6 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kRowCost = 1;
 constexpr int64_t kMostTokens = (int64_t(1) << 31) - 4096;  // token numbers of a chunk past the end still fit in 32 bits
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 struct PagedArgs {
     int B, Hq, Hkv, D, group, tiles, tile_rows;  // group = Hq / Hkv query heads share a key-value head, in `tiles` tiles of tile_rows
@@ -53,7 +52,7 @@ struct PagedArgs {
     // parts: an entry per row where there are fewer rows than blocks, else one per block for the row it began and did not finish
     int part_d;       // D rounded up to a multiple of 4
     float* part_o;    // [2 * blocks][tile_rows][part_d]
-    float2* part_ml;  // [2 * blocks][tile_rows]: maximum (of s log2 e), sum
+    float2* part_ml;  // [2 * blocks][tile_rows]: maximum of the scores, sum
     int4* split;      // {row or -1, its first block, its last block, 0}
     int by_row;
 };
@@ -185,17 +184,26 @@ __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool 
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// Capped and scaled score, in units of log 2: exp(s) = 2^score.
-__device__ __forceinline__ float score_log2(const PagedArgs& a, float dot) {
+// 2^((x - ref) log2 e): the difference is formed first, so that what is rounded by the product is as small as it.
+__device__ __forceinline__ float exp_from(float x, float ref) { return ex2((x - ref) * kLog2e); }
+
+// Scaled and capped score.
+__device__ __forceinline__ float score_of(const PagedArgs& a, float dot) {
     const float s = dot * a.scale;
-    return (a.softcap > 0.f ? a.softcap * tanhf(s / a.softcap) : s) * kLog2e;
+    return a.softcap > 0.f ? a.softcap * tanhf(s / a.softcap) : s;
 }
-// tanh y = 1 - 2 / (e^2y + 1) with an error of 4 * 2^-24 whatever y, against tanhf's 2^-23 relative one: softcap times that lies far
-// below what 16-bit keys leave of a score, and tanhf's two branches took half of the kernel's time. `turn` is 2 log2 e scale / softcap.
-__device__ __forceinline__ float capped_log2(float dot, float turn, float cap_log2e) {
+// The same for 16-bit keys without tanhf's two branches, which took half of the kernel's time: 1 - 2 / (e^2y + 1), off by 4 * 2^-24
+// whatever y, and its series up to y^11, off by 2^-26 of the value, where y is below 0.35 and that would show.
+__device__ __forceinline__ float capped_score(float dot, float per_cap, float cap) {
+    const float y = dot * per_cap, z = y * y;
     float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(ex2(dot * turn) + 1.f));
-    return fmaf(-2.f * cap_log2e, r, cap_log2e);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(ex2(y * (2.f * kLog2e)) + 1.f));
+    float p = fmaf(z, -1382.f / 155925.f, 62.f / 2835.f);
+    p = fmaf(z, p, -17.f / 315.f);
+    p = fmaf(z, p, 2.f / 15.f);
+    p = fmaf(z, p, -1.f / 3.f);
+    p = fmaf(y * z, p, y);
+    return cap * (fabsf(y) < 0.35f ? p : fmaf(-2.f, r, 1.f));
 }
 
 // The four warps' maxima and sums of one query head, and what each warp's output counts in the row's.
@@ -209,11 +217,11 @@ struct Merged {
         sum = 0.f;
 #pragma unroll
         for (int w = 0; w < kWarps; w++) {
-            weight[w] = ex2(ml[w][row].x - ref);
+            weight[w] = exp_from(ml[w][row].x, ref);
             sum = fmaf(weight[w], ml[w][row].y, sum);
         }
     }
-    __device__ __forceinline__ float lse() const { return sum == 0.f ? -INFINITY : top * kLn2 + logf(sum); }
+    __device__ __forceinline__ float lse() const { return sum == 0.f ? -INFINITY : top + logf(sum); }
 };
 
 // ---- 16-bit inputs: tensor cores ---------------------------------------------------------------------------------------------
@@ -344,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) paged_tc_kernel(c
         }
     }
 
-    const float scale_log2e = a.scale * kLog2e, turn = a.softcap > 0.f ? 2.f * scale_log2e / a.softcap : 0.f, cap_log2e = a.softcap * kLog2e;
+    const float per_cap = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
     uint32_t qf[DP / 16][4];
     float acc[NT][4], m[HALVES], l[HALVES];
     int first_chunk = -1, begun = -1, last = 0, stage = 0;
@@ -397,12 +405,12 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) paged_tc_kernel(c
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll
-                    for (int e = 0; e < 2 * HALVES; e++) s[t][e] = capped_log2(s[t][e], turn, cap_log2e);
+                    for (int e = 0; e < 2 * HALVES; e++) s[t][e] = capped_score(s[t][e], per_cap, a.softcap);
             } else {
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll
-                    for (int e = 0; e < 2 * HALVES; e++) s[t][e] *= scale_log2e;
+                    for (int e = 0; e < 2 * HALVES; e++) s[t][e] *= a.scale;
             }
             if (mask != 0xffffu) {
 #pragma unroll
@@ -419,8 +427,8 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) paged_tc_kernel(c
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
                 const float mn = fmaxf(m[r], x);
-                ref[r] = mn == -INFINITY ? 0.f : mn;  // only scores of -inf so far: 2^(-inf - 0) = 0, not a NaN
-                corr[r] = ex2(m[r] - ref[r]);
+                ref[r] = mn == -INFINITY ? 0.f : mn;  // only scores of -inf so far: e^(-inf - 0) = 0, not a NaN
+                corr[r] = exp_from(m[r], ref[r]);
                 moved = moved || m[r] != mn;
                 m[r] = mn;
             }
@@ -443,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) paged_tc_kernel(c
                         s[t][e] = 0.f;
                         continue;
                     }
-                    s[t][e] = ex2(s[t][e] - ref[e >> 1]);
+                    s[t][e] = exp_from(s[t][e], ref[e >> 1]);
                     l[e >> 1] += s[t][e];
                 }
             uint32_t hi[4], lo[4];
@@ -670,12 +678,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_simt_kernel(const T* __rest
                 float x = s[g];
 #pragma unroll
                 for (int o = 1; o < LPK; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-                x = seen ? score_log2(a, x) : -INFINITY;
+                x = seen ? score_of(a, x) : -INFINITY;
                 float t = x;
 #pragma unroll
                 for (int o = LPK; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
                 const float mn = fmaxf(m[g], t), ref = mn == -INFINITY ? 0.f : mn;
-                const float corr = ex2(m[g] - ref), p = ex2(x - ref);
+                const float corr = exp_from(m[g], ref), p = exp_from(x, ref);
                 m[g] = mn;
                 l[g] = l[g] * corr + (sub == 0 ? p : 0.f);
 #pragma unroll
@@ -777,11 +785,11 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(T* __restrict_
     for (int i = lane; i < parts; i += 32) {
         const float2 ml = a.part_ml[part(i)];
         const float next = fmaxf(top, ml.x), ref = next == -INFINITY ? 0.f : next;
-        sum = sum * ex2(top - ref) + ml.y * ex2(ml.x - ref);
+        sum = sum * exp_from(top, ref) + ml.y * exp_from(ml.x, ref);
         top = next;
     }
     const float all = warp_max_f(top), ref = all == -INFINITY ? 0.f : all;
-    sum = warp_sum_f(sum * ex2(top - ref));
+    sum = warp_sum_f(sum * exp_from(top, ref));
 
     const int lanes = width / 4;  // to a part: 8, 16 or 32
     const int d = int(blockIdx.z) * width + (lane & (lanes - 1)) * 4;
@@ -790,7 +798,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(T* __restrict_
 #pragma unroll 2
     for (int i = int(threadIdx.x) / lanes; i < parts; i += int(blockDim.x) / lanes) {
         const float4 x = *reinterpret_cast<const float4*>(columns + int64_t(part(i)) * a.part_d);
-        const float f = ex2(a.part_ml[part(i)].x - ref);
+        const float f = exp_from(a.part_ml[part(i)].x, ref);
         o.x = fmaf(f, x.x, o.x); o.y = fmaf(f, x.y, o.y); o.z = fmaf(f, x.z, o.z); o.w = fmaf(f, x.w, o.w);
     }
 #pragma unroll 1
@@ -807,7 +815,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(T* __restrict_
         for (int w = 0; w < int(blockDim.x >> 5); w++) v += reinterpret_cast<const float*>(sum_s[w])[threadIdx.x];
         O[b * a.os[0] + head * a.os[1] + column] = from_float<T>(sum == 0.f ? 0.f : v / sum);
     }
-    if (a.lse && column == 0) a.lse[b * int64_t(a.Hq) + head] = sum == 0.f ? -INFINITY : all * kLn2 + logf(sum);
+    if (a.lse && column == 0) a.lse[b * int64_t(a.Hq) + head] = sum == 0.f ? -INFINITY : all + logf(sum);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------

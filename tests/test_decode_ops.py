@@ -667,3 +667,47 @@ def test_refusals_with_a_device(rt):
     assert e.value.status == 2
     with pytest.raises(_lib.DoccB200Error):
         ops.token_logprobs(q[0], torch.zeros(4, dtype=torch.int64).cuda(), k=33)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_calls_of_no_extent(rt, dtype):
+    """Empty batches, an empty cache under empty sequences, a table without pages, and no tokens."""
+    empty = lambda *s: torch.empty(*s, dtype=dtype, device="cuda")
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")
+    i64 = lambda n: torch.zeros(n, dtype=torch.int64, device="cuda")
+    assert ops.paged_attention(empty(0, 4, 64), empty(3, 2, 16, 64), empty(3, 2, 16, 64), i32(0, 2), i32(0)).shape == (0, 4, 64)
+    q = normal(2, 4, 64, seed=1, dtype=dtype).cuda()
+    for pages, most in ((0, 0), (0, 3), (3, 0)):
+        out, lse = ops.paged_attention(q, empty(pages, 2, 16, 64), empty(pages, 2, 16, 64), i32(2, most), i32(2), return_lse=True)
+        settle()
+        assert (out == 0).all() and (lse == -math.inf).all()
+    freq = torch.from_numpy(ops.rope_frequencies(64)[0]).cuda()
+    cache = torch.zeros(2, 2, 4, 64, dtype=dtype, device="cuda")
+    assert ops.rope_append(empty(0, 4, 64), empty(0, 2, 64), empty(0, 2, 64), i64(0), freq, cache, cache.clone(), i64(0)).shape == (0, 4, 64)
+    assert ops.rope(empty(0, 4, 64), i64(0), freq).shape == (0, 4, 64) and ops.rope(empty(3, 0, 64), i64(3), freq).shape == (3, 0, 64)
+    assert [t.shape for t in ops.token_logprobs(empty(0, 10), i64(0), k=3)] == [(0,), (0,), (0, 3), (0, 3)]
+    assert ops.rmsnorm(empty(0, 64)).shape == (0, 64) and ops.rmsnorm(empty(4, 0)).shape == (4, 0)
+    assert [t.shape for t in ops.rmsnorm_quant(empty(0, 64), group=128)] == [(0, 64), (0, 1)]
+    with pytest.raises(_lib.DoccB200Error):
+        ops.token_logprobs(empty(2, 0), i64(2))
+    settle()
+
+
+@gpu
+def test_paged_attention_may_write_over_its_query(rt):
+    """A split sequence's parts all read the query before the join writes the output."""
+    q, kc, vc, table, lengths = paged_problem([5000, 3, 0, 700], 8, 2, 64, 16, torch.bfloat16)
+    want = ops.paged_attention(q.cuda(), kc, vc, table.cuda(), lengths.cuda())
+    over = q.cuda()
+    got = ops.paged_attention(over, kc, vc, table.cuda(), lengths.cuda(), out=over)
+    settle()
+    assert got.data_ptr() == over.data_ptr() and torch.equal(over, want)
+
+
+@gpu
+def test_paged_attention_many_sequences(rt):
+    """More sequences than one pass of a warp over the lengths, most of them short."""
+    lengths = [(7 * b) % 50 for b in range(150)]
+    lengths[77] = 2500
+    check_paged(paged_problem(lengths, 2, 1, 64, 8, torch.float16))
