@@ -534,7 +534,9 @@ template <int DP, int GT> struct SimtShape {
     static constexpr int kPieces = DP / 4;                       // 16-byte pieces of a row
     static constexpr int kStage = 2 * kKeys * DP * 4;            // 8 KB
     static constexpr int kStages = 3;
-    static constexpr int kBytes = kWarps * kStages * kStage + (kWarps + 1) * GT * DP * 4;  // the ring, the warps' outputs, the queries
+    // Query heads that are merged at a time: with all eight at DP = 128 the block had 117 KB and an SM room for one instead of two.
+    static constexpr int kMerge = GT < 4 ? GT : 4;
+    static constexpr int kBytes = kWarps * kStages * kStage + (kWarps * kMerge + GT) * DP * 4;  // the ring, the outputs, the queries
     static __device__ __forceinline__ int offset(int row, int piece) {  // in floats; eight lanes of a step read eight banks
         return row * DP + ((piece ^ ((row * kLanes) & 7)) << 2);
     }
@@ -553,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_simt_kernel(const T* __rest
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     float* ring = reinterpret_cast<float*>(smem + warp * (S * Shape::kStage));
     float* merge = reinterpret_cast<float*>(smem + kWarps * S * Shape::kStage);
-    float* q_s = merge + kWarps * GT * DP;
+    float* q_s = merge + kWarps * Shape::kMerge * DP;
     if (a.D < DP) {
         for (int i = lane; i < S * Shape::kStage / 4; i += 32) ring[i] = 0.f;
         __syncwarp();
@@ -719,34 +721,40 @@ __global__ void __launch_bounds__(kThreads, 2) paged_simt_kernel(const T* __rest
         }
         const bool row_done = at.chunk + 1 == at.chunks;
         if (row_done || at.left == 1) {
-            float* mine = merge + warp * (GT * DP);
+            constexpr int M = Shape::kMerge;
+            float* mine = merge + warp * (M * DP);
 #pragma unroll
             for (int g = 0; g < GT; g++) {
                 l[g] = warp_sum_f(l[g]);
                 if (lane == 0) ml_s[warp][g] = make_float2(m[g], l[g]);
-#pragma unroll
-                for (int c = 0; c < C; c++) mine[g * DP + (C == 2 ? lane * 2 + c : (c >> 2) * 128 + lane * 4 + (c & 3))] = acc[g][c];
             }
             const bool whole = first_chunk == 0 && row_done;
             const int64_t part = 2 * int64_t(blockIdx.x) + (first_chunk == 0 ? 1 : 0);
-            __syncthreads();
-            for (int i = threadIdx.x; i < GT * DP; i += kThreads) {
-                const int g = i / DP, d = i % DP, in_group = at.tile * GT + g;
-                if (in_group >= a.group) break;
-                const Merged all(ml_s, g);
-                float o = 0.f;
 #pragma unroll
-                for (int w = 0; w < kWarps; w++) o = fmaf(all.weight[w], merge[w * (GT * DP) + i], o);
-                const int64_t head = int64_t(at.kvh) * a.group + in_group;
-                if (whole) {
-                    if (d < a.D) O[at.b * a.os[0] + head * a.os[1] + d] = from_float<T>(all.sum == 0.f ? 0.f : o / all.sum);
-                    if (a.lse && d == 0) a.lse[at.b * int64_t(a.Hq) + head] = all.lse();
-                } else {
-                    if (d < a.D) a.part_o[(part * a.tile_rows + g) * a.part_d + d] = o;
-                    if (d == 0) a.part_ml[part * a.tile_rows + g] = make_float2(all.top, all.sum);
+            for (int g0 = 0; g0 < GT; g0 += M) {
+#pragma unroll
+                for (int g = 0; g < M; g++)
+#pragma unroll
+                    for (int c = 0; c < C; c++) mine[g * DP + (C == 2 ? lane * 2 + c : (c >> 2) * 128 + lane * 4 + (c & 3))] = acc[g0 + g][c];
+                __syncthreads();
+                for (int i = threadIdx.x; i < M * DP; i += kThreads) {
+                    const int g = g0 + i / DP, d = i % DP, in_group = at.tile * GT + g;
+                    if (in_group >= a.group) break;
+                    const Merged all(ml_s, g);
+                    float o = 0.f;
+#pragma unroll
+                    for (int w = 0; w < kWarps; w++) o = fmaf(all.weight[w], merge[w * (M * DP) + i], o);
+                    const int64_t head = int64_t(at.kvh) * a.group + in_group;
+                    if (whole) {
+                        if (d < a.D) O[at.b * a.os[0] + head * a.os[1] + d] = from_float<T>(all.sum == 0.f ? 0.f : o / all.sum);
+                        if (a.lse && d == 0) a.lse[at.b * int64_t(a.Hq) + head] = all.lse();
+                    } else {
+                        if (d < a.D) a.part_o[(part * a.tile_rows + g) * a.part_d + d] = o;
+                        if (d == 0) a.part_ml[part * a.tile_rows + g] = make_float2(all.top, all.sum);
+                    }
                 }
+                __syncthreads();  // the buffers are the next heads' or the next row's
             }
-            __syncthreads();
             if (first_chunk == 0) {
                 if (!whole) {
                     begun = row_of(a, at);

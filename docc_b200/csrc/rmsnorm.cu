@@ -15,7 +15,7 @@ namespace docc_b200 {
 namespace {
 
 constexpr int64_t kRmsMaxCols = 32768;  // the row is staged in shared memory in fp32: 128 KB of 227
-constexpr int kRmsGroup = 128, kRmsLoads = 4;
+constexpr int kRmsGroup = 128, kRmsLoads = 4, kRmsWarpCols = 1024;
 constexpr float kE4m3Max = 448.f;
 
 // Maximum that keeps a NaN, so that a group holding one gets a NaN scale instead of a plausible one.
@@ -177,31 +177,38 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR == 128 ? 8 : 1) rms
 // element with an 8-bit output): 1021 rows of 5003 take 9.8 us, a quarter of the copy rate. The same in registers, unrolled over 20
 // columns per thread, has half as many instructions and took 19.8 us: they no longer fit the instruction cache. On the 16-byte packs
 // of the whole matrix, gamma moved into place by selects, it took 10.8.
-template <typename T, bool Q8>
+// TPR threads to a row: a block, or a warp.
+template <typename T, bool Q8, int TPR>
 __global__ void __launch_bounds__(256) rmsnorm_row_kernel(const T* X, const T* R, T* S, T* Y, uint8_t* Q, float* scales, RmsArgs a) {
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
-    extern __shared__ float row_s[];
+    constexpr int RPB = 256 / TPR, WPR = TPR / 32;
+    extern __shared__ float rows_s[];
     __shared__ float red[8];
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int t = threadIdx.x % TPR, lane = t & 31, warp = t >> 5;
     const int cols = int(a.cols);
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    float* row_s = rows_s + int(threadIdx.x / TPR) * cols;
+    auto sync = [] {
+        if constexpr (WPR > 1) __syncthreads();
+        else __syncwarp();
+    };
+    for (int64_t row = int64_t(blockIdx.x) * RPB + threadIdx.x / TPR; row < a.rows; row += int64_t(gridDim.x) * RPB) {
         const T* x = X + row * a.ldx;
         const T* r = R ? R + row * a.ldr : nullptr;
         float ss = 0.f;
-        for (int c0 = t; c0 < cols; c0 += 256 * kRmsLoads) {  // all loads of a round before the first use
+        for (int c0 = t; c0 < cols; c0 += TPR * kRmsLoads) {  // all loads of a round before the first use
             T vx[kRmsLoads], vr[kRmsLoads];
 #pragma unroll
             for (int i = 0; i < kRmsLoads; i++)
-                if (c0 + i * 256 < cols) vx[i] = x[c0 + i * 256];
+                if (c0 + i * TPR < cols) vx[i] = x[c0 + i * TPR];
             if (r) {
 #pragma unroll
                 for (int i = 0; i < kRmsLoads; i++)
-                    if (c0 + i * 256 < cols) vr[i] = r[c0 + i * 256];
+                    if (c0 + i * TPR < cols) vr[i] = r[c0 + i * TPR];
             }
 #pragma unroll
             for (int i = 0; i < kRmsLoads; i++) {
-                const int c = c0 + i * 256;
+                const int c = c0 + i * TPR;
                 if (c >= cols) break;
                 const float v = r ? to_float(vx[i]) + to_float(vr[i]) : to_float(vx[i]);
                 row_s[c] = v;
@@ -209,53 +216,55 @@ __global__ void __launch_bounds__(256) rmsnorm_row_kernel(const T* X, const T* R
                 ss = fmaf(v, v, ss);
             }
         }
-        const float rstd = rsqrtf(block_sum_f(ss, red) / float(cols) + a.eps);
+        if constexpr (WPR > 1) ss = block_sum_f(ss, red);
+        else ss = warp_sum_f(ss);
+        const float rstd = rsqrtf(ss / float(cols) + a.eps);
         if constexpr (!Q8) {
-            for (int c = t; c < cols; c += 256) {
+            for (int c = t; c < cols; c += TPR) {
                 const float y = row_s[c] * rstd;
                 Y[row * a.cols + c] = from_float<T>(a.gamma ? y * a.gamma[c] : y);
             }
-        } else {
-            // a group per warp in turn; a whole-row group is the one group of warp 0..7 together
-            const int64_t groups = (a.cols + a.group - 1) / a.group;
-            if (a.group >= a.cols) {
-                float m = 0.f;
-                for (int c = t; c < cols; c += 256) {
-                    const float y = a.gamma ? row_s[c] * rstd * a.gamma[c] : row_s[c] * rstd;
-                    row_s[c] = y;
-                    m = max_nan(m, fabsf(y));
-                }
-                m = warp_max_nan(m);
+        } else if (a.group >= a.cols) {
+            float m = 0.f;
+            for (int c = t; c < cols; c += TPR) {
+                const float y = a.gamma ? row_s[c] * rstd * a.gamma[c] : row_s[c] * rstd;
+                row_s[c] = y;
+                m = max_nan(m, fabsf(y));
+            }
+            m = warp_max_nan(m);
+            if constexpr (WPR > 1) {
                 __syncthreads();
                 if (lane == 0) red[warp] = m;
                 __syncthreads();
                 m = red[0];
-                for (int w = 1; w < 8; w++) m = max_nan(m, red[w]);
-                const Quantiser by(m);
-                for (int c = t; c < cols; c += 256) Q[row * a.cols + c] = by.one(row_s[c]);
-                if (t == 0) scales[row] = by.scale;
-            } else {
-                for (int g = warp; g < groups; g += 8) {
-                    const int c0 = int(g * a.group), c1 = int(c0 + a.group < a.cols ? c0 + a.group : a.cols);
-                    float y[kRmsGroup / 32], m = 0.f;
+                for (int w = 1; w < WPR; w++) m = max_nan(m, red[w]);
+            }
+            const Quantiser by(m);
+            for (int c = t; c < cols; c += TPR) Q[row * a.cols + c] = by.one(row_s[c]);
+            if (t == 0) scales[row] = by.scale;
+        } else {  // a group per warp in turn
+            sync();
+            const int64_t groups = (a.cols + a.group - 1) / a.group;
+            for (int g = warp; g < groups; g += WPR) {
+                const int c0 = int(g * a.group), c1 = int(c0 + a.group < a.cols ? c0 + a.group : a.cols);
+                float y[kRmsGroup / 32], m = 0.f;
 #pragma unroll
-                    for (int i = 0; i < kRmsGroup / 32; i++) {
-                        const int c = c0 + lane + 32 * i;
-                        y[i] = 0.f;
-                        if (c < c1) y[i] = a.gamma ? row_s[c] * rstd * a.gamma[c] : row_s[c] * rstd;
-                        m = max_nan(m, fabsf(y[i]));
-                    }
-                    const Quantiser by(warp_max_nan(m));
-#pragma unroll
-                    for (int i = 0; i < kRmsGroup / 32; i++) {
-                        const int c = c0 + lane + 32 * i;
-                        if (c < c1) Q[row * a.cols + c] = by.one(y[i]);
-                    }
-                    if (lane == 0) scales[row * groups + g] = by.scale;
+                for (int i = 0; i < kRmsGroup / 32; i++) {
+                    const int c = c0 + lane + 32 * i;
+                    y[i] = 0.f;
+                    if (c < c1) y[i] = a.gamma ? row_s[c] * rstd * a.gamma[c] : row_s[c] * rstd;
+                    m = max_nan(m, fabsf(y[i]));
                 }
+                const Quantiser by(warp_max_nan(m));
+#pragma unroll
+                for (int i = 0; i < kRmsGroup / 32; i++) {
+                    const int c = c0 + lane + 32 * i;
+                    if (c < c1) Q[row * a.cols + c] = by.one(y[i]);
+                }
+                if (lane == 0) scales[row * groups + g] = by.scale;
             }
         }
-        __syncthreads();  // row_s and red are reused by the next row
+        sync();  // row_s and red are reused by the next row
     }
 }
 
@@ -266,6 +275,19 @@ int launch_rms(Ctx* ctx, const RmsArgs& a, const void* X, const void* R, void* S
                              static_cast<const T*>(X), static_cast<const T*>(R), static_cast<T*>(S), static_cast<T*>(Y),
                              static_cast<uint8_t*>(Q), static_cast<float*>(scales), a));
     return after_launch(ctx, "rmsnorm_kernel");
+}
+
+template <typename T, bool Q8, int TPR>
+int launch_rms_row(Ctx* ctx, const RmsArgs& a, const void* X, const void* R, void* S, void* Y, void* Q, void* scales) {
+    constexpr int RPB = 256 / TPR;
+    const size_t smem = size_t(a.cols) * 4 * RPB;
+    auto kernel = rmsnorm_row_kernel<T, Q8, TPR>;
+    if (smem > 48 * 1024) DOCC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+    const int64_t cap = int64_t(ctx->sm_count) * 8, blocks = ceil_div(a.rows, RPB);
+    const int grid = int(blocks < cap ? blocks : cap);
+    DOCC_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(256), smem, ctx->stream, static_cast<const T*>(X), static_cast<const T*>(R),
+                             static_cast<T*>(S), static_cast<T*>(Y), static_cast<uint8_t*>(Q), static_cast<float*>(scales), a));
+    return after_launch(ctx, "rmsnorm_row_kernel");
 }
 
 template <typename T, bool Q8>
@@ -284,14 +306,10 @@ int rms_device(Ctx* ctx, const RmsArgs& a, const void* X, const void* R, void* S
         if (packs <= 2048) return launch_rms<T, Q8, 512, 4>(ctx, a, X, R, S, Y, Q, scales);
         if (packs <= 4096) return launch_rms<T, Q8, 1024, 4>(ctx, a, X, R, S, Y, Q, scales);
     }
-    const size_t smem = size_t(a.cols) * 4;
-    auto kernel = rmsnorm_row_kernel<T, Q8>;
-    if (smem > 48 * 1024) DOCC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
-    const int64_t cap = int64_t(ctx->sm_count) * 8;
-    const int grid = int(a.rows < cap ? a.rows : cap);
-    DOCC_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(256), smem, ctx->stream, static_cast<const T*>(X), static_cast<const T*>(R),
-                             static_cast<T*>(S), static_cast<T*>(Y), static_cast<uint8_t*>(Q), static_cast<float*>(scales), a));
-    return after_launch(ctx, "rmsnorm_row_kernel");
+    // a warp per row where rows are short and enough to fill the SMs with warps: 9195 rows of 182 6.4 us against 22.0 with a block each,
+    // 20000 of 801 35 against 75, but 300 of 501 4.7 against 2.7, and 5000 of 1501 without codes 24 against 15
+    if (a.cols <= kRmsWarpCols && a.rows >= 8 * int64_t(ctx->sm_count)) return launch_rms_row<T, Q8, 32>(ctx, a, X, R, S, Y, Q, scales);
+    return launch_rms_row<T, Q8, 256>(ctx, a, X, R, S, Y, Q, scales);
 }
 
 int rms_any(Ctx* ctx, int prec, const RmsArgs& a, const void* X, const void* R, void* S, void* Y, void* Q, void* scales) {

@@ -53,7 +53,7 @@ def rms_tolerance(y, cols):
 
 
 RMS_SHAPES = [(1, 1), (1, 7), (3, 64), (5, 127), (2, 128), (4, 129), (7, 257), (3, 1000), (33, 1024), (2, 4096), (3, 5003), (2, 8200),
-              (2, 16384), (1, 32768), (300, 512), (1500, 256)]
+              (2, 16384), (1, 32768), (300, 512), (1500, 256), (1300, 333), (1200, 1023)]
 
 
 @gpu
