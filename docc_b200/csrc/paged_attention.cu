@@ -527,7 +527,9 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) paged_tc_kernel(c
 
 // ---- fp32, and whatever is not aligned for 16-byte copies: FMA units -------------------------------------------------------------
 // A warp step is KS keys, 32 / KS lanes to a key for the scores and DP / 32 columns to a lane for the output; keys and values are
-// staged as fp32. Up to GT query heads share the step.
+// staged as fp32. Up to GT query heads share the step. With one head per key-value head the stream bounds it (16 sequences of 16
+// heads of 128: 63 us for a floor of 56; of 64: 22 for 15); with several, the query's and the values' trips through shared memory
+// do, at 8 warps to an SM: 16 sequences with 4 heads to a key-value head of 128 take 55 us for a floor of 28, 16 to one of 80 60 for 9.
 template <int DP, int GT> struct SimtShape {
     static constexpr int kKeys = 1024 / DP;                      // 16, 8, 4
     static constexpr int kLanes = 32 / kKeys;                    // lanes per key
@@ -552,6 +554,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_simt_kernel(const T* __rest
     __shared__ float2 ml_s[kWarps][GT];
     __shared__ uint32_t mask_s[kWarps][S];
     __shared__ __align__(16) float p_s[kWarps][GT][KS];
+    __shared__ float corr_s[kWarps][GT];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     float* ring = reinterpret_cast<float*>(smem + warp * (S * Shape::kStage));
     float* merge = reinterpret_cast<float*>(smem + kWarps * S * Shape::kStage);
@@ -626,7 +629,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_simt_kernel(const T* __rest
         }
     }
 
-    float acc[GT][C], m[GT], l[GT];
+    // A lane's scores are those of GL query heads from `own` on, of one key; DUP lanes hold the same one.
+    constexpr int GL = GT > LPK ? GT / LPK : 1, DUP = LPK > GT ? LPK / GT : 1;
+    const int my_key = lane / LPK, sub = lane % LPK, own = sub / DUP * GL;
+    float acc[GT][C], m[GL], l[GL];
     int first_chunk = -1, begun = -1, last = 0, stage = 0;
     do {
         if (first_chunk < 0) {
@@ -640,11 +646,13 @@ __global__ void __launch_bounds__(kThreads, 2) paged_simt_kernel(const T* __rest
             }
             __syncthreads();
 #pragma unroll
-            for (int g = 0; g < GT; g++) {
+            for (int g = 0; g < GT; g++)
 #pragma unroll
                 for (int c = 0; c < C; c++) acc[g][c] = 0.f;
-                m[g] = -INFINITY;
-                l[g] = 0.f;
+#pragma unroll
+            for (int i = 0; i < GL; i++) {
+                m[i] = -INFINITY;
+                l[i] = 0.f;
             }
         }
         if constexpr (ASYNC) cp_async_wait<S - 2>();
@@ -659,7 +667,6 @@ __global__ void __launch_bounds__(kThreads, 2) paged_simt_kernel(const T* __rest
         if (mask) {
             const float* kb = ring + stage * (Shape::kStage / 4);
             const float* vb = kb + KS * DP;
-            const int my_key = lane / LPK, sub = lane % LPK;
             float s[GT];
 #pragma unroll
             for (int g = 0; g < GT; g++) s[g] = 0.f;
@@ -674,25 +681,49 @@ __global__ void __launch_bounds__(kThreads, 2) paged_simt_kernel(const T* __rest
                 }
             }
             const bool seen = (mask >> my_key) & 1;
-            __syncwarp();  // p_s of the step before has been read
+            // The lanes of a key add up their shares and divide the heads among themselves on the way: each step sends the half of the
+            // heads that the other lane keeps. Cap, exponential and maximum are then taken once per key and head, not once per lane.
 #pragma unroll
-            for (int g = 0; g < GT; g++) {
-                float x = s[g];
+            for (int o = LPK / 2, n = GT; o > 0; o >>= 1) {
+                if (n > 1) {
+                    n >>= 1;
 #pragma unroll
-                for (int o = 1; o < LPK; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-                x = seen ? score_of(a, x) : -INFINITY;
-                float t = x;
-#pragma unroll
-                for (int o = LPK; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
-                const float mn = fmaxf(m[g], t), ref = mn == -INFINITY ? 0.f : mn;
-                const float corr = exp_from(m[g], ref), p = exp_from(x, ref);
-                m[g] = mn;
-                l[g] = l[g] * corr + (sub == 0 ? p : 0.f);
-#pragma unroll
-                for (int c = 0; c < C; c++) acc[g][c] *= corr;
-                if (sub == 0) p_s[warp][g][my_key] = p;
+                    for (int i = 0; i < GT / 2; i++) {
+                        if (i >= n) break;
+                        const bool upper = sub & o;
+                        const float give = upper ? s[i] : s[i + n], keep = upper ? s[i + n] : s[i];
+                        s[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+                    }
+                } else {
+                    s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
+                }
             }
+            __syncwarp();  // p_s and corr_s of the step before have been read
+            bool moved = false;
+#pragma unroll
+            for (int i = 0; i < GL; i++) {
+                const float x = seen ? score_of(a, s[i]) : -INFINITY;
+                float top = x;
+#pragma unroll
+                for (int o = LPK; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const float mn = fmaxf(m[i], top), ref = mn == -INFINITY ? 0.f : mn;
+                const float corr = exp_from(m[i], ref), p = exp_from(x, ref);
+                moved = moved || m[i] != mn;
+                m[i] = mn;
+                l[i] = l[i] * corr + (sub % DUP == 0 ? p : 0.f);
+                if (sub % DUP == 0) p_s[warp][own + i][my_key] = p;
+                if (lane < LPK && sub % DUP == 0) corr_s[warp][own + i] = corr;
+            }
+            const bool any_moved = __any_sync(0xffffffffu, moved);
             __syncwarp();
+            if (any_moved) {
+#pragma unroll
+                for (int g = 0; g < GT; g++) {
+                    const float corr = corr_s[warp][g];
+#pragma unroll
+                    for (int c = 0; c < C; c++) acc[g][c] *= corr;
+                }
+            }
 #pragma unroll
             for (int j4 = 0; j4 < KS / 4; j4++) {
                 float v[4][C];
@@ -724,9 +755,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_simt_kernel(const T* __rest
             constexpr int M = Shape::kMerge;
             float* mine = merge + warp * (M * DP);
 #pragma unroll
-            for (int g = 0; g < GT; g++) {
-                l[g] = warp_sum_f(l[g]);
-                if (lane == 0) ml_s[warp][g] = make_float2(m[g], l[g]);
+            for (int i = 0; i < GL; i++) {
+#pragma unroll
+                for (int o = LPK; o < 32; o <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
+                if (lane < LPK && sub % DUP == 0) ml_s[warp][own + i] = make_float2(m[i], l[i]);
             }
             const bool whole = first_chunk == 0 && row_done;
             const int64_t part = 2 * int64_t(blockIdx.x) + (first_chunk == 0 ? 1 : 0);
