@@ -3,7 +3,7 @@
 Each function accepts either numpy arrays (host memory: the call stages the data
 through the device, docc's "WithTransfers" flavour) or torch CUDA tensors (device
 pointers, asynchronous on the library's current stream). Mixed inputs are an error.
-Outputs have the kind of the inputs.
+Outputs have the kind of the inputs. All calls are forward: outputs carry no gradient.
 
 Stream ordering of device calls: the library's current stream is, by default, a private
 non-blocking stream of the calling thread that is NOT ordered after torch's streams. Code that
