@@ -361,6 +361,7 @@ __global__ void __launch_bounds__(BLOCK, 1024 / BLOCK) logprobs_kernel(const T* 
         Sums all = join_lanes<WARPS>(sums_s[lane % WARPS]);
 
         if constexpr (TOP) {
+            key = max(key, ordered(-INFINITY));  // a later bar may be a -inf: the threads that have nothing else hold those, too
             while (true) {
                 if (key >= uint32_t(bar >> 32)) streams_s[atomicAdd(&n_streams, 1)] = t;
                 __syncthreads();

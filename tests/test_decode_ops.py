@@ -711,3 +711,43 @@ def test_paged_attention_many_sequences(rt):
     lengths = [(7 * b) % 50 for b in range(150)]
     lengths[77] = 2500
     check_paged(paged_problem(lengths, 2, 1, 64, 8, torch.float16))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [2, 700])
+def test_token_logprobs_when_very_many_logits_compete(rt, rows, dtype):
+    """Rows in which more logits reach the first bound than are kept at a time: all equal, two values, all but three masked out."""
+    vocab = 131072 if rows == 2 else 9000
+    x = torch.zeros(rows, vocab, dtype=dtype)
+    x[1, ::3] = 1.0
+    if rows > 2:
+        x[2::7] = -float("inf")
+        x[2::7, 4000:4003] = torch.tensor([1.0, 5.0, 1.0], dtype=dtype)
+        x[3::7, 1000:] = 2.0
+    check_logprobs(x, torch.full((rows,), 4001), 32)
+    check_logprobs(x, torch.full((rows,), 4001), 1)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_token_logprobs_of_rows_full_of_nan(rt, dtype):
+    x = normal(3, 30001, seed=3, dtype=dtype)
+    x[0, 5000:] = float("nan")
+    x[1, 7::2] = float("nan")
+    x[2, 1234] = float("inf")
+    logp, entropy, top_ids, top_logp = ops.token_logprobs(x.cuda(), torch.tensor([1, 2, 1234]).cuda(), k=4)
+    settle()
+    assert torch.isnan(logp).all() and torch.isnan(entropy).all() and torch.isnan(top_logp).all()
+    assert top_ids[0].tolist() == [5000, 5001, 5002, 5003] and top_ids[1].tolist() == [7, 9, 11, 13] and top_ids[2, 0] == 1234
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,allowed", [(1, 131072, 1), (3, 128001, 3), (40, 50021, 19), (160, 32000, 2), (600, 128000, 5)])
+def test_token_logprobs_when_a_mask_leaves_fewer_tokens_than_asked(rt, rows, vocab, allowed, dtype):
+    """The masked tokens fill the list in the order of their indices, with a log-probability of -inf."""
+    x = torch.full((rows, vocab), -float("inf"), dtype=dtype)
+    at = torch.randint(vocab, (rows, allowed), generator=torch.Generator().manual_seed(rows))
+    x.scatter_(1, at, normal(rows, allowed, seed=vocab, dtype=dtype))
+    check_logprobs(x, at[:, 0], 20)
