@@ -271,7 +271,7 @@ PyObject* token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
     int64_t rows, vocab, ld, k;
     double scale;
     if (!x || !ids || x->dim() != 2 || !precision(*x) || !rows_of(*x, rows, vocab, ld) || !vector_of(*ids, at::kLong, rows) || !whole(args[2], k) ||
-        k < 0 || !number(args[3], scale))
+        k < 0 || k > 32 || !number(args[3], scale))
         Py_RETURN_NONE;
     const Tensor logp = empty({rows}, *x, at::kFloat), entropy = empty({rows}, *x, at::kFloat);
     const Tensor top_ids = empty({rows, k}, *x, at::kLong), top_logp = empty({rows, k}, *x, at::kFloat);

@@ -734,7 +734,8 @@ def token_logprobs(logits, ids, k=0, scale=1.0, flags=0):
         logp, entropy = _new(logits, (2, rows), "float32").unbind(0)
     else:
         logp, entropy = _new(logits, (rows,), "float32"), _new(logits, (rows,), "float32")
-    top_ids, top_logp = _new(ids, (rows, k)), _new(logits, (rows, k), "float32")
+    width = k if 0 <= k <= 32 else 0  # nothing is allocated for a k that the call refuses
+    top_ids, top_logp = _new(ids, (rows, width)), _new(logits, (rows, width), "float32")
     call("docc_b200_token_logprobs", _prec(logits), rows, vocab, _addr(logits), ldx, scale, _addr(ids), _addr(logp), _addr(entropy), k,
          _addr(top_ids), _addr(top_logp), flags)
     return logp, entropy, top_ids, top_logp

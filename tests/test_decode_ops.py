@@ -618,6 +618,21 @@ def test_refusals_of_host_calls():
         ops.token_logprobs(f, pos)
 
 
+@pytest.mark.parametrize("k", [-1, 9, 33, 10**15])
+def test_token_logprobs_refuses_a_k_without_allocating_for_it(k):
+    with pytest.raises(_lib.DoccB200Error) as e:
+        ops.token_logprobs(np.zeros((2, 8), dtype=np.float32), np.zeros(2, dtype=np.int64), k=k)
+    assert e.value.status == 1
+
+
+@gpu
+@pytest.mark.parametrize("k", [-1, 9, 33, 10**15])
+def test_token_logprobs_refuses_a_k_on_the_device(rt, k):
+    with pytest.raises(_lib.DoccB200Error) as e:
+        ops.token_logprobs(torch.zeros(2, 8, device="cuda"), torch.zeros(2, dtype=torch.int64).cuda(), k=k)
+    assert e.value.status == 1
+
+
 def status_of(name, *args):
     return getattr(_lib.lib(), name)(*args)
 
