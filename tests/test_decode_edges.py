@@ -1,0 +1,80 @@
+"""Edges of the decoding-step operators that their other tests do not reach: values at the middle between two 8-bit codes, one key far
+above all others, visible infinities, rows around the shared memory that needs no opt-in, a failing call's status, and a host side that
+could not be built."""
+import math
+import os
+import subprocess
+import sys
+import threading
+
+import numpy as np
+import pytest
+import torch
+
+from docc_b200 import _lib, ops
+from test_decode_ops import DTYPES, E, TINY, U, attention_exact, close, gpu, normal, paged_problem, rms_exact, rms_tolerance, settle
+
+# ---- 8-bit codes ------------------------------------------------------------------------------------------------------------------
+def e4m3_middles():
+    """The values half way between two neighbouring codes, from the smallest on."""
+    codes = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    return (codes[1:] + codes[:-1]) / 2
+
+
+def codes_problem(cols, tops, seed):
+    """gamma whose quotients by its groups' scales lie at the middles between two codes and up to three steps of fp32 beside them.
+    Signs as an input have a mean square of exactly 1, so the norm is the signed gamma, bit for bit."""
+    rng = np.random.default_rng(seed)
+    width = -(-cols // len(tops))
+    gamma = np.zeros(cols, dtype=np.float32)
+    for i, top in enumerate(np.float32(tops)):
+        part = gamma[i * width : (i + 1) * width]
+        scale = top / np.float32(448)
+        y = (scale.astype(np.float64) * rng.choice(e4m3_middles().numpy(), len(part))).astype(np.float32)
+        for _ in range(3):
+            y = np.where(rng.random(len(part)) < 0.4, np.nextafter(y, np.float32(rng.choice([0, 1e38]))), y)
+        part[:] = np.minimum(y, top)
+        part[0] = top
+    return torch.from_numpy(gamma)
+
+
+def codes_of(y, group):
+    """scale = max|y| / 448 and e4m3(y / scale), each rounded once from fp32 operands; a scale of 0 has codes of 0."""
+    scales, codes = [], []
+    for part in y.split(y.shape[1] if group == 0 else 128, dim=1):
+        scale = part.abs().amax(1, keepdim=True) / 448
+        q = torch.where(scale > 0, part / scale, 0.0).clamp(-448, 448)
+        scales.append(scale)
+        codes.append(q.to(torch.float8_e4m3fn))
+    return torch.cat([c.view(torch.uint8) for c in codes], 1), torch.cat(scales, 1)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("group", [0, 128])
+@pytest.mark.parametrize("rows,cols", [(3, 256), (5, 1024), (2, 4096), (2, 8192), (3, 257), (4, 1001), (2, 5003), (1300, 333), (1200, 1022)])
+def test_codes_are_those_of_the_quotient(rt, rows, cols, group, dtype):
+    """Bit for bit where y / scale lies at the middle between two codes or a step beside it: the quotient decides, not a product with a
+    rounded reciprocal."""
+    tops = [1.7] if group == 0 else [1.7 + 0.37 * i for i in range(-(-cols // 128))]
+    gamma = codes_problem(cols, tops, seed=rows + cols)
+    x = torch.where(normal(rows, cols, seed=cols) < 0, -1.0, 1.0)
+    q, scales = ops.rmsnorm_quant(x.to(dtype).cuda(), gamma.cuda(), eps=0.0, group=group)
+    settle()
+    want, want_scales = codes_of(x * gamma, group)
+    assert torch.equal(scales.cpu(), want_scales)
+    assert torch.equal(q.cpu().view(torch.uint8), want)
+
+
+@gpu
+@pytest.mark.parametrize("cols", [1024, 1021])
+def test_codes_under_tiny_scales(rt, cols):
+    """Scales below fp32's smallest normal number, whose own rounding is large, one that rounds to zero, and a group of zeros."""
+    tops = [1.5, 3e-30, 1e-38, 448 * 2.0**-140, 5 * 2.0**-141, 2.0**-149, 0.0, 1e-42]
+    gamma = codes_problem(cols, tops, seed=cols)
+    x = torch.where(normal(3, cols, seed=1) < 0, -1.0, 1.0)
+    q, scales = ops.rmsnorm_quant(x.cuda(), gamma.cuda(), eps=0.0, group=128)
+    settle()
+    want, want_scales = codes_of(x * gamma, 128)
+    assert torch.equal(scales.cpu(), want_scales)
+    assert torch.equal(q.cpu().float(), want.view(torch.float8_e4m3fn).float())  # -0 and 0 are one value
