@@ -230,6 +230,9 @@ struct Merged {
 // over, while the 128-row accumulators of tcgen05 would be 8/128 full and pay the trip through tensor memory on every step.
 // Q stays in registers, K comes as B fragments by ldmatrix, P goes from accumulator to A operand without leaving the registers.
 // P enters the product as two 16-bit parts (p = hi + lo): a single bf16 would add an error as large as the output's own rounding.
+// fp16 takes P times 2^15, which the output is divided by at the merge: both parts end at fp16's smallest step, 2^-24, and without the
+// factor 8192 keys 18 below one that dominates, together a probability of 1e-4 each 1.5e-8, lost a fifth of their share. 1 becomes
+// 32768, inside fp16's range, and what is lost is below 2^-40 of the largest probability. The sum needs no factor: it is fp32.
 template <typename T> __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if constexpr (std::is_same<T, __half>::value)
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -279,6 +282,8 @@ template <int DP> struct TcShape {
         return uint32_t(row * kRow + ((piece ^ turn) << 4));
     }
 };
+
+template <typename T> constexpr float kLift = std::is_same<T, __half>::value ? 0x1p15f : 1.f;
 
 // HALVES: 1 where the tile has at most eight query heads (rows 8-15 of the fragments are padding), else 2.
 template <typename T, int DP, int HALVES>
@@ -457,8 +462,8 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) paged_tc_kernel(c
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                split2<T>(s[t][0], s[t][1], hi[2 * t], lo[2 * t]);
-                split2<T>(s[t][2], s[t][3], hi[2 * t + 1], lo[2 * t + 1]);
+                split2<T>(s[t][0] * kLift<T>, s[t][1] * kLift<T>, hi[2 * t], lo[2 * t]);
+                split2<T>(s[t][2] * kLift<T>, s[t][3] * kLift<T>, hi[2 * t + 1], lo[2 * t + 1]);
             }
 #pragma unroll
             for (int i = 0; i < NT / 2; i++) {
@@ -485,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) paged_tc_kernel(c
 #pragma unroll
                 for (int i = 0; i < NT; i++)
                     *reinterpret_cast<float2*>(merge + Shape::merged(warp, lane >> 2, i * 8 + (lane & 3) * 2)) =
-                        make_float2(acc[i][2 * r], acc[i][2 * r + 1]);
+                        make_float2(acc[i][2 * r] * (1.f / kLift<T>), acc[i][2 * r + 1] * (1.f / kLift<T>));
                 __syncthreads();
                 const int d = (threadIdx.x % (DP / 2)) * 2;
                 for (int g = threadIdx.x / (DP / 2); g < 8; g += kThreads / (DP / 2)) {

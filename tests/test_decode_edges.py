@@ -78,3 +78,38 @@ def test_codes_under_tiny_scales(rt, cols):
     want, want_scales = codes_of(x * gamma, 128)
     assert torch.equal(scales.cpu(), want_scales)
     assert torch.equal(q.cpu().float(), want.view(torch.float8_e4m3fn).float())  # -0 and 0 are one value
+# ---- attention: one key far above the others --------------------------------------------------------------------------------------
+def sink_problem(B, length, gap, group, kv, dim, dtype, page=16, seed=0):
+    """Sequences that share their pages: the first key scores ``gap`` above the others, which lie around 0, and its value is zero."""
+    pages = -(-length // page)
+    kc, vc = torch.zeros(pages, kv, page, dim, dtype=dtype), 1 + 0.1 * normal(pages, kv, page, dim, seed=seed).to(dtype)
+    kc[..., 0] = (0.1 * normal(pages, kv, page, seed=seed + 1)).to(dtype)
+    kc[0, :, 0, 0] = gap
+    vc[0, :, 0] = 0
+    q = torch.zeros(1, group * kv, dim, dtype=dtype)
+    q[..., 0] = 1
+    table = torch.arange(pages, dtype=torch.int32)[None]
+    lengths = torch.tensor([length], dtype=torch.int32)
+    got = ops.paged_attention(q.expand(B, -1, -1).contiguous().cuda(), kc.cuda(), vc.cuda(), table.expand(B, -1).contiguous().cuda(),
+                              lengths.expand(B).contiguous().cuda(), scale=1.0, return_lse=True)
+    settle()
+    want = attention_exact(q, kc, vc, table, lengths, 1.0, 0.0, 0)
+    for g, w, tol in ((got[0], want[0], want[1]), (got[1], want[2], want[3])):
+        close(g, w.expand(g.shape), tol.expand(g.shape))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gap", [16.0, 17.5, 20.0, 24.0])
+@pytest.mark.parametrize("whole", [True, False])
+def test_attention_keeps_small_probabilities(rt, whole, gap, dtype):
+    """Thousands of keys whose probabilities, each below the smallest number of fp16, make up the whole output: a row per block, and one
+    row split over all blocks."""
+    blocks = 2 * torch.cuda.get_device_properties(0).multi_processor_count
+    sink_problem(blocks if whole else 1, 8192, gap, 1, 1, 64, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("group,kv,dim", [(4, 2, 80), (16, 1, 128), (12, 2, 64), (2, 1, 256), (20, 1, 96)])
+def test_attention_keeps_small_probabilities_in_every_kernel(rt, group, kv, dim):
+    sink_problem(3, 3000, 19.0, group, kv, dim, torch.float16, seed=5)
