@@ -258,14 +258,22 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float x, float y
         return *reinterpret_cast<const uint32_t*>(&h);
     }
 }
-// hi = the pair rounded to 16 bits, lo = what the rounding left, rounded
+// hi = the pair rounded to 16 bits towards zero, lo = what that left, rounded. Neither is negative, and lo is at least the type's
+// smallest number (fp16: smallest step) where hi is not 0, so that an infinite value times the two gives twice that infinity: 0 inf
+// or the difference of two infinities would be a NaN.
 template <typename T> __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-    hi = pack2<T>(x, y);
+    uint32_t least;
     if constexpr (std::is_same<T, __half>::value) {
+        asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(y), "f"(x));
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
         lo = pack2<T>(x - f.x, y - f.y);
+        asm("min.f16x2 %0, %1, %2;" : "=r"(least) : "r"(hi), "r"(0x00010001u));
+        asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(lo) : "r"(least));
     } else {
+        asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(y), "f"(x));
         lo = pack2<T>(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
+        asm("min.bf16x2 %0, %1, %2;" : "=r"(least) : "r"(hi), "r"(0x00800080u));
+        asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(lo) : "r"(least));
     }
 }
 

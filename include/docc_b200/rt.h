@@ -300,7 +300,10 @@ int docc_b200_rope_append(int prec, int64_t tokens, int64_t Hq, int64_t Hkv, int
  * max(0, n - window) <= j < n of sequence b, n = lengths[b] (window 0: all). softcap c > 0 replaces
  * s by c * tanh(s / c). Token j lies at place j % page_size of page page_table[b * table_stride +
  * j / page_size]; query head h reads key-value head h / (Hq / Hkv). lse (fp32 [B, Hq], may be NULL)
- * receives log sum_j exp(s_j). A sequence without visible tokens gives O = 0 and lse = -inf.
+ * receives log sum_j exp(s_j). A sequence without visible tokens gives O = 0 and lse = -inf. What is
+ * not visible may hold anything. An infinite V of a visible token makes its column of O infinite (two of
+ * opposite sign, or a NaN, a NaN), unless its p is below 2^-126 of the sequence's largest (prec 'h':
+ * 2^-39), where it may also give a NaN.
  * lengths and page_table are int32 in device memory, read when the kernel runs. A length outside
  * [0, max_pages * page_size] is clamped and the tokens of a page number outside [0, num_pages) are
  * left out; both are reported by docc_b200_sync as DOCC_B200_ERR_BAD_INDEX.

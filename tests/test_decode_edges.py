@@ -113,3 +113,42 @@ def test_attention_keeps_small_probabilities(rt, whole, gap, dtype):
 @pytest.mark.parametrize("group,kv,dim", [(4, 2, 80), (16, 1, 128), (12, 2, 64), (2, 1, 256), (20, 1, 96)])
 def test_attention_keeps_small_probabilities_in_every_kernel(rt, group, kv, dim):
     sink_problem(3, 3000, 19.0, group, kv, dim, torch.float16, seed=5)
+# ---- attention: infinities that are seen ------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lengths,heads", [([1, 2, 40, 700], 4), ([5000, 33], 16)])
+def test_attention_of_a_visible_infinite_value(rt, lengths, heads, dtype):
+    """p inf = inf for every p > 0, in its own column only; two of opposite sign, or a NaN, give a NaN."""
+    q, kc, vc, table, lengths = paged_problem(lengths, heads, 1, 64, 16, dtype)
+    settle()
+    plain = ops.paged_attention(q.cuda(), kc, vc, table.cuda(), lengths.cuda())
+    settle()
+    bad = {5: [math.inf], 9: [-math.inf], 20: [math.inf, -math.inf], 31: [math.nan]}
+    want = plain.clone()
+    for b, n in enumerate(lengths.tolist()):
+        for column, values in bad.items():
+            if len(values) > n:
+                continue
+            for i, v in enumerate(values):
+                j = (n - 1 - 7 * i) % n
+                vc[int(table[b, j // 16]), 0, j % 16, column] = v
+            want[b, :, column] = sum(values)
+    settle()
+    got = ops.paged_attention(q.cuda(), kc, vc, table.cuda(), lengths.cuda())
+    settle()
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0.0, 1e4, -1e4), want.nan_to_num(0.0, 1e4, -1e4))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_of_an_infinite_value_of_small_probability(rt, dtype):
+    """A key far below the one that dominates still has a probability, and so an infinite share."""
+    gap = 26.0 if dtype == torch.float16 else 85.0  # e^-26 = 2^-37.5, e^-85 = 2^-122.6
+    kc, vc = torch.zeros(1, 1, 16, 64, dtype=dtype, device="cuda"), torch.ones(1, 1, 16, 64, dtype=dtype, device="cuda")
+    kc[0, 0, 3, 0], vc[0, 0, 7, 2] = gap, math.inf
+    q = torch.zeros(1, 2, 64, dtype=dtype, device="cuda")
+    q[..., 0] = 1
+    settle()
+    got = ops.paged_attention(q, kc, vc, torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.tensor([16], dtype=torch.int32).cuda(), scale=1.0)
+    settle()
+    assert (got[..., 2] == math.inf).all() and (got[..., :2] == 1).all() and (got[..., 3:] == 1).all()
