@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -137,6 +138,16 @@ inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+// Lets a kernel have up to `bytes` of dynamic shared memory, a constant: a launch with less never lowers what another thread's launch
+// needs. Without it static and dynamic memory together end at 48 KB. Set once per kernel and device: `done` is the caller's, one per kernel.
+template <typename F> int set_smem(Ctx* ctx, std::atomic<unsigned>& done, F kernel, int bytes) {
+    const unsigned bit = 1u << ctx->device;  // fewer than 16 devices
+    if (done.load(std::memory_order_acquire) & bit) return DOCC_B200_OK;
+    DOCC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(bit, std::memory_order_release);
+    return DOCC_B200_OK;
 }
 
 }  // namespace docc_b200

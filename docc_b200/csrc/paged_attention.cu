@@ -20,7 +20,6 @@
 // the first chunk's way through lengths, page table and keys 3, the join 8 with its launch; one of 1025: 9.8 us. In an early form the
 // median block of the first case was done after 102 us and the slowest, with a run of short rows, after 142: hence kRowCost. More runs
 // than resident blocks gained nothing (147, 155 and 166 us with 2, 4 and 8 times as many).
-#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -887,15 +886,6 @@ Scratch scratch_of(int blocks, int64_t group, int64_t D) {
     return s;
 }
 int blocks_of(Ctx* ctx, int64_t D) { return ctx->sm_count * (D <= 128 ? 2 : 1); }
-
-// The attribute is set once per kernel and device: `done` is the caller's, one per kernel.
-template <typename F> int set_smem(Ctx* ctx, std::atomic<unsigned>& done, F kernel, int bytes) {
-    const unsigned bit = 1u << ctx->device;  // fewer than 16 devices
-    if (done.load(std::memory_order_acquire) & bit) return DOCC_B200_OK;
-    DOCC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    done.fetch_or(bit, std::memory_order_release);
-    return DOCC_B200_OK;
-}
 
 template <typename T>
 int launch_join(Ctx* ctx, const PagedArgs& a, int blocks, T* O) {

@@ -320,7 +320,8 @@ int launch_rms_row(Ctx* ctx, const RmsArgs& a, const void* X, const void* R, voi
     constexpr int RPB = 256 / TPR;
     const size_t smem = size_t(a.cols) * 4 * RPB;
     auto kernel = rmsnorm_row_kernel<T, Q8, TPR>;
-    if (smem > 48 * 1024) DOCC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+    static std::atomic<unsigned> done{0};
+    DOCC_TRY(set_smem(ctx, done, kernel, int((TPR == 32 ? kRmsWarpCols : kRmsMaxCols) * 4 * RPB)));
     const int64_t cap = int64_t(ctx->sm_count) * 8, blocks = ceil_div(a.rows, RPB);
     const int grid = int(blocks < cap ? blocks : cap);
     DOCC_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(256), smem, ctx->stream, static_cast<const T*>(X), static_cast<const T*>(R),

@@ -152,3 +152,67 @@ def test_attention_of_an_infinite_value_of_small_probability(rt, dtype):
     got = ops.paged_attention(q, kc, vc, torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.tensor([16], dtype=torch.int32).cuda(), scale=1.0)
     settle()
     assert (got[..., 2] == math.inf).all() and (got[..., :2] == 1).all() and (got[..., 3:] == 1).all()
+# ---- RMS norm: rows around the 48 KB of shared memory that need no opt-in ---------------------------------------------------------
+def norm_of_width(cols, dtype, quant, offset=0, rows=2):
+    flat = normal(rows * cols + offset, seed=cols, dtype=dtype)
+    x = flat[offset:].view(rows, cols)
+    on_device = flat.cuda()[offset:].view(rows, cols)
+    if quant:
+        q, scales = ops.rmsnorm_quant(on_device, eps=1e-6)
+        ops.sync()
+        got = q.float().double().cpu() * scales.double().cpu()
+        _, y = rms_exact(x, None, None, 1e-6)
+        drift = (cols / 32 + 20) * E
+        close(got, y, y.abs() * (2.0**-4 + 4 * drift) + y.abs().amax(1, keepdim=True) / 448 * 2.0**-10 * (1 + 4 * drift))
+    else:
+        got = ops.rmsnorm(on_device, eps=1e-6)
+        ops.sync()
+        _, y = rms_exact(x, None, None, 1e-6)
+        close(got, y, y.abs() * U[dtype] * 1.01 + rms_tolerance(y, cols) + TINY[dtype])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("quant", [False, True])
+def test_rmsnorm_of_widths_beside_48_kb(rt, quant, dtype):
+    for cols, offset in ((12281, 0), (12287, 0), (12288, 1), (12289, 0), (32767, 0), (12283, 0)):
+        norm_of_width(cols, dtype, quant, offset)
+
+
+@gpu
+def test_rmsnorm_of_such_a_width_is_the_first_call(rt):
+    """In a process of its own, where no wider row has been seen before."""
+    code = ("import torch, test_decode_edges as t; from docc_b200 import ops; ops.init(0); "
+            "ops.set_stream(torch.cuda.current_stream().cuda_stream); "
+            "[t.norm_of_width(12281, d, q) for d in t.DTYPES for q in (False, True)]; print('done')")
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([os.path.dirname(__file__), os.path.dirname(os.path.dirname(__file__))]))
+    got = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0 and "done" in got.stdout, got.stderr[-2000:]
+
+
+@gpu
+def test_rmsnorm_of_two_widths_from_two_threads(rt):
+    """Neither thread's rows change what the other's kernel may use."""
+    xs = [normal(2, cols, seed=cols, dtype=torch.bfloat16).cuda() for cols in (12301, 32767)]
+    torch.cuda.synchronize()
+    want = [ops.rmsnorm(x) for x in xs]
+    settle()
+    wrong = []
+
+    def work(i):
+        try:
+            ops.init(0)
+            for _ in range(300):
+                got = ops.rmsnorm(xs[i])
+                ops.sync()
+                if not torch.equal(got, want[i]):
+                    wrong.append(i)
+        except Exception as e:  # noqa: BLE001
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i % 2,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
