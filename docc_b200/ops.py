@@ -404,7 +404,7 @@ def _compiled(x):
         loader = ExtensionFileLoader("docc_b200_decode_calls", HOST_PATH)
         module = module_from_spec(spec_from_loader(loader.name, loader))
         loader.exec_module(module)
-        module.bind(*(ctypes.cast(getattr(_lib.lib(), name), _vp).value for name in _NATIVE))
+        module.bind(*(ctypes.cast(getattr(_lib.lib(), name), _vp).value for name in _NATIVE), _lib.check)
         _native = module
     return _native
 

@@ -1,6 +1,7 @@
 """Edges of the decoding-step operators that their other tests do not reach: values at the middle between two 8-bit codes, one key far
 above all others, visible infinities, rows around the shared memory that needs no opt-in, a failing call's status, and a host side that
 could not be built."""
+import ctypes
 import math
 import os
 import subprocess
@@ -216,3 +217,48 @@ def test_rmsnorm_of_two_widths_from_two_threads(rt):
     for t in threads:
         t.join()
     assert not wrong
+# ---- the compiled host side: statuses ---------------------------------------------------------------------------------------------
+def ordinary_calls():
+    """A call of every entry that the compiled host side takes."""
+    x, pos, freq = torch.zeros(2, 4, 64, device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda"), torch.zeros(32, dtype=torch.float64, device="cuda")
+    cache, table, lengths = torch.zeros(3, 4, 16, 64, device="cuda"), torch.zeros(2, 1, dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    return {"docc_b200_rmsnorm": lambda: ops.rmsnorm(x), "docc_b200_rmsnorm_q8": lambda: ops.rmsnorm_quant(x),
+            "docc_b200_rope": lambda: ops.rope(x, pos, freq, out=x),
+            "docc_b200_rope_append": lambda: ops.rope_append(x, x, x, pos, freq, cache, cache, pos, out=x),
+            "docc_b200_paged_attention": lambda: ops.paged_attention(x, cache, cache, table, lengths),
+            "docc_b200_token_logprobs": lambda: ops.token_logprobs(x[:, 0], pos, k=2)}
+
+
+def bound_to(entries):
+    """Binds the compiled host side to ``entries`` where given, to the library's own otherwise."""
+    module = ops._compiled(torch.zeros(1))
+    address = lambda name: ctypes.cast(entries.get(name, getattr(_lib.lib(), name)), ctypes.c_void_p).value
+    module.bind(*(address(name) for name in ops._NATIVE), _lib.check)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["docc_b200_rmsnorm", "docc_b200_rmsnorm_q8", "docc_b200_rope", "docc_b200_rope_append", "docc_b200_paged_attention",
+                                  "docc_b200_token_logprobs"])
+def test_a_call_that_failed_is_not_made_again(rt, name):
+    """A status that may come after the kernel was queued raises from the one call; rotated in place, a second one would turn twice."""
+    restype, argtypes = _lib.SIGNATURES[name]
+    calls = []
+    entry = ctypes.CFUNCTYPE(restype, *argtypes)(lambda *args: calls.append(args) or status)
+    run = ordinary_calls()[name]
+    rt.docc_b200_launch_count(1)
+    try:
+        bound_to({name: entry})
+        for status in (3, 4, 5, 6):  # CUDA, out of memory, no device, timeout
+            calls.clear()
+            with pytest.raises(_lib.DoccB200Error) as e:
+                run()
+            assert e.value.status == status and name in str(e.value) and len(calls) == 1
+        assert rt.docc_b200_launch_count(0) == 0
+        for status in (1, 2):  # refused before anything was queued: the Python side makes the call, and here it succeeds
+            calls.clear()
+            run()
+            assert len(calls) == 1
+        assert rt.docc_b200_launch_count(0) >= 2
+    finally:
+        bound_to({})
+    settle()
