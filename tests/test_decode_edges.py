@@ -7,6 +7,7 @@ import os
 import subprocess
 import sys
 import threading
+import time
 
 import numpy as np
 import pytest
@@ -262,3 +263,26 @@ def test_a_call_that_failed_is_not_made_again(rt, name):
     finally:
         bound_to({})
     settle()
+@gpu
+def test_other_threads_run_while_an_entry_waits(rt):
+    """The entry stands for one that waits for a stream: the C library's poll(fds, 0, cols), which sleeps ``cols`` milliseconds and
+    returns 0, in the place of rmsnorm(prec, 0 rows, cols, ...)."""
+    x = torch.empty(0, 400, device="cuda")
+    stop, ticks = threading.Event(), []
+
+    def tick():
+        while not stop.wait(0.002):
+            ticks.append(time.monotonic())
+
+    thread = threading.Thread(target=tick)
+    try:
+        bound_to({"docc_b200_rmsnorm": ctypes.CDLL(None).poll})
+        thread.start()
+        begin = time.monotonic()
+        ops.rmsnorm(x)
+        end = time.monotonic()
+    finally:
+        bound_to({})
+        stop.set()
+        thread.join()
+    assert end - begin >= 0.39 and len([t for t in ticks if begin < t < end]) >= 20
