@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-import os
+import warnings
 
 import numpy as np
 
@@ -384,12 +384,12 @@ def _addr(x):
 
 _NATIVE = ("docc_b200_rmsnorm", "docc_b200_rmsnorm_q8", "docc_b200_rope", "docc_b200_rope_append", "docc_b200_paged_attention",
            "docc_b200_token_logprobs")
-_native = None  # the compiled form of these calls for torch tensors (docc_b200/host); None until the first of them
+_native = None  # the compiled form of these calls for torch tensors (docc_b200/host): None until the first of them, False if there is none
 
 
 def _compiled(x):
     """The module that takes the ordinary call on torch tensors; it answers None to every other, which then runs here. False before the
-    first torch tensor has been met."""
+    first torch tensor has been met, and where the module has not been built for this torch and interpreter."""
     global _native
     if _native is None:
         if not _is_torch(x):
@@ -397,13 +397,20 @@ def _compiled(x):
         from importlib.machinery import ExtensionFileLoader
         from importlib.util import module_from_spec, spec_from_loader
 
-        from .build import HOST_PATH
+        from .build import HOST_NAME, host_path
 
-        if not os.path.exists(HOST_PATH):
-            raise RuntimeError(f"{HOST_PATH} is missing: run `python -m docc_b200.build`.")
-        loader = ExtensionFileLoader("docc_b200_decode_calls", HOST_PATH)
-        module = module_from_spec(spec_from_loader(loader.name, loader))
-        loader.exec_module(module)
+        path = host_path()
+        if path is None:  # a tensor type of another package
+            return False
+        try:
+            loader = ExtensionFileLoader(HOST_NAME, path)
+            module = module_from_spec(spec_from_loader(loader.name, loader))
+            loader.exec_module(module)
+        except ImportError as e:
+            warnings.warn(f"{path} cannot be loaded ({e}): these calls take their Python path, which is 4-13 us slower. "
+                          "Run `python -m docc_b200.build`.", RuntimeWarning, stacklevel=3)
+            _native = False
+            return False
         module.bind(*(ctypes.cast(getattr(_lib.lib(), name), _vp).value for name in _NATIVE), _lib.check)
         _native = module
     return _native

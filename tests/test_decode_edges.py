@@ -8,12 +8,13 @@ import subprocess
 import sys
 import threading
 import time
+import warnings
 
 import numpy as np
 import pytest
 import torch
 
-from docc_b200 import _lib, ops
+from docc_b200 import _lib, build, ops
 from test_decode_ops import DTYPES, E, TINY, U, attention_exact, close, gpu, normal, paged_problem, rms_exact, rms_tolerance, settle
 
 # ---- 8-bit codes ------------------------------------------------------------------------------------------------------------------
@@ -286,3 +287,54 @@ def test_other_threads_run_while_an_entry_waits(rt):
         stop.set()
         thread.join()
     assert end - begin >= 0.39 and len([t for t in ticks if begin < t < end]) >= 20
+# ---- the compiled host side: where it cannot be built -----------------------------------------------------------------------------
+@pytest.mark.parametrize("compiler", ["false", "/no/such/compiler"])
+def test_the_runtime_is_built_where_the_host_side_cannot_be(monkeypatch, tmp_path, compiler):
+    """A box with torch but without its compiler or the interpreter's headers; what an earlier build left there is not kept."""
+    monkeypatch.setattr(build, "LIB_DIR", str(tmp_path))
+    monkeypatch.setattr(build, "_build_runtime", lambda verbose: None)
+    monkeypatch.setenv("CXX", compiler)
+    with open(build.host_path(), "w") as fh:
+        fh.write("built by another compiler")
+    with pytest.warns(RuntimeWarning, match="could not be compiled"):
+        assert build.build() == build.LIB_PATH
+    assert not os.path.exists(build.host_path()) and not build.host_is_current()
+
+
+def test_the_host_side_belongs_to_one_torch_and_interpreter(monkeypatch):
+    here = build.host_path()
+    assert build.host_is_current() and os.path.exists(here)
+    with monkeypatch.context() as m:
+        m.setattr(build, "_torch_version", lambda: "0.1")
+        assert build.host_path() != here and not build.host_is_current()
+    with monkeypatch.context() as m:
+        m.setattr(build.sysconfig, "get_config_var", lambda name: "cpython-999")
+        assert build.host_path() != here and not build.host_is_current()
+    with monkeypatch.context() as m:
+        m.setattr(build, "_torch_root", lambda: None)  # no torch, no host side
+        assert build.host_path() is None and build.host_is_current()
+
+
+def test_calls_without_the_compiled_host_side(monkeypatch):
+    """They take the Python path, which says what is wrong, and warn once."""
+    monkeypatch.setattr(ops, "_native", None)
+    monkeypatch.setattr(build, "_torch_version", lambda: "0.1")
+    with pytest.warns(RuntimeWarning, match="cannot be loaded"):
+        with pytest.raises(TypeError, match="CUDA device"):
+            ops.rmsnorm(torch.zeros(2, 8))
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        with pytest.raises(TypeError, match="CUDA device"):
+            ops.token_logprobs(torch.zeros(2, 8), torch.zeros(2, dtype=torch.int64))
+
+
+@gpu
+def test_results_without_the_compiled_host_side(rt, monkeypatch):
+    x = normal(5, 300, seed=1).cuda()
+    want = ops.rmsnorm(x)
+    monkeypatch.setattr(ops, "_native", None)
+    monkeypatch.setattr(build, "_torch_version", lambda: "0.1")
+    with pytest.warns(RuntimeWarning, match="cannot be loaded"):
+        got = ops.rmsnorm(x)
+    settle()
+    assert torch.equal(got, want)
