@@ -74,8 +74,10 @@ struct Ctx {
     cudaStream_t copy_streams[2] = {nullptr, nullptr};
     cudaEvent_t copy_events[4] = {nullptr, nullptr, nullptr, nullptr};
     cudaEvent_t switch_event = nullptr;  // orders a newly selected stream after the one it replaces
-    void* workspace[4] = {nullptr, nullptr, nullptr, nullptr};  // library-owned scratch, grows on demand
-    size_t workspace_bytes[4] = {0, 0, 0, 0};
+    // Library-owned scratch, grows on demand. Slots 0-3 may be part of a captured graph; slot 4 is the paged attention's, which never is.
+    static constexpr int kWorkspaces = 5;
+    void* workspace[kWorkspaces] = {};
+    size_t workspace_bytes[kWorkspaces] = {};
     DeviceStatus* status_host = nullptr;  // mapped pinned
     DeviceStatus* status_dev = nullptr;   // device alias of status_host
     int sm_count = 0;

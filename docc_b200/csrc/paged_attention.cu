@@ -1020,7 +1020,7 @@ extern "C" int docc_b200_paged_attention(int prec, int64_t B, int64_t Hq, int64_
         cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
         DOCC_CUDA_TRY(cudaStreamIsCapturing(ctx->stream, &capture));
         DOCC_REQUIRE(capture == cudaStreamCaptureStatusNone, "paged_attention: a captured call needs a workspace of its own");
-        DOCC_TRY(get_workspace(ctx, 3, scratch.bytes, &workspace));
+        DOCC_TRY(get_workspace(ctx, 4, scratch.bytes, &workspace));
     }
     PagedArgs a;
     a.B = int(B); a.Hq = int(Hq); a.Hkv = int(Hkv); a.D = int(D); a.group = int(Hq / Hkv);

@@ -271,7 +271,7 @@ int docc_b200_shutdown(void) {
     Ctx* c = &tls_ctx[dev & 15];
     if (c->device != dev) return DOCC_B200_OK;
     DOCC_CUDA_TRY(cudaStreamSynchronize(c->stream));
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < Ctx::kWorkspaces; i++) {
         if (c->workspace[i]) pool_free(c->workspace[i]);
         c->workspace[i] = nullptr;
         c->workspace_bytes[i] = 0;

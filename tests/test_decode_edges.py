@@ -338,3 +338,35 @@ def test_results_without_the_compiled_host_side(rt, monkeypatch):
         got = ops.rmsnorm(x)
     settle()
     assert torch.equal(got, want)
+# ---- scratch ----------------------------------------------------------------------------------------------------------------------
+@gpu
+def test_the_cache_attention_leaves_the_scratch_of_a_captured_attention_alone(rt):
+    """fp32 attention over contiguous keys may be captured with the thread's scratch; an eager call over the cache that needs more than
+    that must neither use the same memory nor give it back."""
+    changed = []
+
+    def work():  # a new thread has scratch of its own, which begins empty
+        try:
+            ops.init(0)
+            stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+            ops.set_stream(stream.cuda_stream)
+            with torch.cuda.stream(stream):
+                q = normal(1, 2, 256, 64, seed=1).cuda()
+                want = ops.attention(q, q, q)
+                with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
+                    got = ops.attention(q, q, q)
+                paged = paged_problem([3000], 16, 1, 128, 16, torch.bfloat16)
+                out = ops.paged_attention(paged[0].cuda(), paged[1], paged[2], paged[3].cuda(), paged[4].cuda())
+                held = [ops.DeviceArray.from_numpy(np.full(100_000, 7, dtype=np.float32)) for _ in range(8)]
+                graph.replay()
+                stream.synchronize()
+                changed.extend(i for i, h in enumerate(held) if not (h.to_numpy() == 7).all())
+                changed.extend([] if torch.equal(got, want) and torch.isfinite(out).all() else ["result"])
+            ops.sync()
+        except Exception as e:  # noqa: BLE001
+            changed.append(e)
+
+    thread = threading.Thread(target=work)
+    thread.start()
+    thread.join()
+    assert not changed
