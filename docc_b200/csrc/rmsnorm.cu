@@ -372,7 +372,13 @@ int rms_checked(const char* what, int prec, const RmsArgs& a, const void* X, con
     DOCC_REQUIRE(a.eps >= 0.f, "%s: eps must not be negative", what);
     Ctx* ctx;
     DOCC_TRY(get_ctx(&ctx));
-    if (a.rows == 0 || a.cols == 0) return DOCC_B200_OK;
+    if (a.rows == 0 || a.cols == 0) {
+        if (a.rows == 0 || a.group != 0 || !scales) return DOCC_B200_OK;
+        // a scale per row: rows of nothing have scales of 0
+        if (flags & DOCC_B200_FLAG_HOST_PTRS) memset(scales, 0, size_t(a.rows) * 4);
+        else DOCC_CUDA_TRY(cudaMemsetAsync(scales, 0, size_t(a.rows) * 4, ctx->stream));
+        return DOCC_B200_OK;
+    }
     DOCC_REQUIRE(X && (Y || (Q && scales)), "%s: NULL data pointer", what);
     DOCC_REQUIRE(a.ldx >= a.cols && (!R || a.ldr >= a.cols), "%s: row stride below cols", what);
     if (a.cols > kRmsMaxCols) return set_error(DOCC_B200_ERR_UNSUPPORTED, "%s: cols %lld > %lld", what, (long long)a.cols, (long long)kRmsMaxCols);

@@ -264,7 +264,8 @@ int docc_b200_rmsnorm(int prec, int64_t rows, int64_t cols, const void* X, int64
 /* The same norm y with an 8-bit output: columns are taken in groups of `group` (128, or 0 for the
  * whole row; the last group may be shorter), scale = max|y| / 448 of the group in fp32, and
  * Q = e4m3(y / scale), the fp32 quotient rounded to nearest even. A group of zeros, or of values so
- * small that their scale rounds to 0, has scale 0 and Q 0; a group that holds a NaN has scale NaN. Q: rows x cols bytes; scales: rows x ceil(cols / group) fp32. */
+ * small that their scale rounds to 0, has scale 0 and Q 0; a group that holds a NaN has scale NaN. Q: rows x cols bytes; scales: rows x ceil(cols / group) fp32, with group 0
+ * one per row (0 where cols is 0). */
 int docc_b200_rmsnorm_q8(int prec, int64_t rows, int64_t cols, const void* X, int64_t ldx,
                          const void* residual, int64_t ldr, const void* gamma, double eps,
                          int64_t group, void* S, void* Q, void* scales, int flags);

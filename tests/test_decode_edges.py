@@ -370,3 +370,17 @@ def test_the_cache_attention_leaves_the_scratch_of_a_captured_attention_alone(rt
     thread.start()
     thread.join()
     assert not changed
+# ---- outputs of calls without elements --------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scales_of_rows_of_nothing(rt, dtype):
+    """One scale per row is a row's even if it has no columns: zero, like that of a row of zeros."""
+    for _ in range(4):
+        used = torch.full((5, 1), 7.0, device="cuda")
+        settle()
+        del used  # the next allocation of this size is likely to hold sevens
+        q, scales = ops.rmsnorm_quant(torch.empty(5, 0, dtype=dtype, device="cuda"), group=0)
+        settle()
+        assert q.shape == (5, 0) and scales.shape == (5, 1) and (scales == 0).all()
+    assert ops.rmsnorm_quant(torch.empty(5, 0, dtype=dtype, device="cuda"), group=128)[1].shape == (5, 0)
+    assert (ops.rmsnorm_quant(np.empty((5, 0), dtype=np.float32))[1] == 0).all()
