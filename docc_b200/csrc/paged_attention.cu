@@ -1001,7 +1001,11 @@ extern "C" int docc_b200_paged_attention(int prec, int64_t B, int64_t Hq, int64_
         return set_error(DOCC_B200_ERR_UNSUPPORTED, "paged_attention: the cache lives on the device; host pointers are not taken");
     Ctx* ctx;
     DOCC_TRY(get_ctx(&ctx));
-    if (B == 0 || Hq == 0 || D == 0) return DOCC_B200_OK;
+    if (B == 0 || Hq == 0) return DOCC_B200_OK;
+    if (D == 0) {
+        DOCC_REQUIRE(!lse, "paged_attention: heads of no elements have no lse");
+        return DOCC_B200_OK;
+    }
     DOCC_REQUIRE(Hkv > 0 && Hq % Hkv == 0, "paged_attention: %lld query heads are not a multiple of %lld key-value heads", (long long)Hq,
                  (long long)Hkv);
     if (D > 256) return set_error(DOCC_B200_ERR_UNSUPPORTED, "paged_attention: head_dim %lld > 256", (long long)D);

@@ -308,7 +308,8 @@ int docc_b200_rope_append(int prec, int64_t tokens, int64_t Hq, int64_t Hkv, int
  * lengths and page_table are int32 in device memory, read when the kernel runs. A length outside
  * [0, max_pages * page_size] is clamped and the tokens of a page number outside [0, num_pages) are
  * left out; both are reported by docc_b200_sync as DOCC_B200_ERR_BAD_INDEX.
- * Strides: Q, O [sb,sh]; caches [sp,sh,ss] as above; NULL = contiguous. D <= 256, prec 's', 'b', 'h'.
+ * Strides: Q, O [sb,sh]; caches [sp,sh,ss] as above; NULL = contiguous. D <= 256 (0: nothing is written,
+ * and lse must be NULL), prec 's', 'b', 'h'.
  * The scratch holds partial results of sequences that several blocks share. workspace == NULL uses
  * the calling thread's own (ordered on its stream); a captured call has to bring its own, of
  * docc_b200_paged_attention_workspace() bytes, so that graphs which run at the same time do not

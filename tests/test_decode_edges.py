@@ -384,3 +384,13 @@ def test_scales_of_rows_of_nothing(rt, dtype):
         assert q.shape == (5, 0) and scales.shape == (5, 1) and (scales == 0).all()
     assert ops.rmsnorm_quant(torch.empty(5, 0, dtype=dtype, device="cuda"), group=128)[1].shape == (5, 0)
     assert (ops.rmsnorm_quant(np.empty((5, 0), dtype=np.float32))[1] == 0).all()
+@gpu
+def test_attention_of_heads_without_elements_has_no_lse(rt):
+    """Its scores would be those of empty products; the call that would have to return them is refused."""
+    q, cache = torch.empty(2, 4, 0, device="cuda"), torch.empty(3, 2, 16, 0, device="cuda")
+    table, lengths = torch.zeros(2, 1, dtype=torch.int32).cuda(), torch.ones(2, dtype=torch.int32).cuda()
+    assert ops.paged_attention(q, cache, cache, table, lengths).shape == (2, 4, 0)
+    with pytest.raises(_lib.DoccB200Error) as e:
+        ops.paged_attention(q, cache, cache, table, lengths, return_lse=True)
+    assert e.value.status == 1
+    settle()
