@@ -394,3 +394,37 @@ def test_attention_of_heads_without_elements_has_no_lse(rt):
         ops.paged_attention(q, cache, cache, table, lengths, return_lse=True)
     assert e.value.status == 1
     settle()
+# ---- arrays of the runtime's own pool ---------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_calls_on_arrays_of_the_pool(rt, dtype):
+    """A whole step on DeviceArrays gives DeviceArrays that hold what torch tensors give."""
+    held = lambda t: ops.DeviceArray.from_numpy(t.cpu().numpy())
+    same = lambda a, t: isinstance(a, ops.DeviceArray) and np.array_equal(a.to_numpy(), t.cpu().numpy())
+    x, gamma, res = normal(4, 256, seed=1, dtype=dtype).cuda(), 1 + 0.1 * normal(256, seed=2).cuda(), normal(4, 256, seed=3, dtype=dtype).cuda()
+    both = [(ops.rmsnorm(held(x), held(gamma)),), (ops.rmsnorm(x, gamma),)]
+    both[0] += ops.rmsnorm(held(x), held(gamma), held(res))
+    both[1] += ops.rmsnorm(x, gamma, res)
+    codes = ops.rmsnorm_quant(held(x), held(gamma), held(res), group=128)
+    want = ops.rmsnorm_quant(x, gamma, res, group=128)
+    both[0] += codes
+    both[1] += (want[0].view(torch.uint8), *want[1:])
+    q, k, v = normal(4, 8, 64, seed=4, dtype=dtype).cuda(), normal(4, 2, 64, seed=5, dtype=dtype).cuda(), normal(4, 2, 64, seed=6, dtype=dtype).cuda()
+    pos, freq = torch.arange(4).cuda() + 900, torch.from_numpy(ops.rope_frequencies(32)[0]).cuda()
+    kc, vc, slots = torch.zeros(3, 2, 16, 64, dtype=dtype).cuda(), torch.zeros(3, 2, 16, 64, dtype=dtype).cuda(), torch.tensor([0, 17, 18, -1]).cuda()
+    table, lengths = torch.tensor([[0, 1], [1, 0], [1, 2], [2, 0]], dtype=torch.int32).cuda(), torch.tensor([20, 3, 5, 0], dtype=torch.int32).cuda()
+    both[0] += (ops.rope(held(q), held(pos), held(freq), interleaved=True, mscale=1.5),)
+    both[1] += (ops.rope(q, pos, freq, interleaved=True, mscale=1.5),)
+    dk, dv = held(kc), held(vc)
+    both[0] += (ops.rope_append(held(q), held(k), held(v), held(pos), held(freq), dk, dv, held(slots)), dk, dv)
+    both[1] += (ops.rope_append(q, k, v, pos, freq, kc, vc, slots), kc, vc)
+    settle()
+    both[0] += ops.paged_attention(held(q), dk, dv, held(table), held(lengths), window=9, return_lse=True)
+    both[1] += ops.paged_attention(q, kc, vc, table, lengths, window=9, return_lse=True)
+    ids = torch.tensor([0, 255, 3, -1]).cuda()
+    got, want = ops.token_logprobs(held(x), held(ids), k=4), ops.token_logprobs(x, ids, k=4)
+    settle()
+    for a, t in zip(*both):
+        assert same(a, t)
+    for a, t in zip(got, want):
+        assert isinstance(a, ops.DeviceArray) and np.array_equal(a.to_numpy(), t.cpu().numpy(), equal_nan=a.dtype.kind == "f")
