@@ -16,8 +16,8 @@
 //     sum: nothing synchronises but the merge of the four warps at the end of a row.
 //
 // Measured (bf16 / fp16, heads of 128, fresh inputs per call): 64 ragged sequences up to 8192 tokens, 32 heads on 8, 609 MB: 116 us
-// (5.2 TB/s, 0.80 of the measured copy); one of 131079 tokens, 16 heads on 2, capped scores, 134 MB: 36.5 us, of which the stream is 25,
-// the first chunk's way through lengths, page table and keys 3, the join 8 with its launch; one of 1025: 9.8 us. In an early form the
+// (5.2 TB/s, 0.80 of the measured copy); one of 131079 tokens, 16 heads on 2, capped scores, 134 MB: 37.2 us, of which the stream is 25,
+// the first chunk's way through lengths, page table and keys 3, the join 8 with its launch; one of 1025: 10.0 us. In an early form the
 // median block of the first case was done after 102 us and the slowest, with a run of short rows, after 142: hence kRowCost. More runs
 // than resident blocks gained nothing (147, 155 and 166 us with 2, 4 and 8 times as many).
 #include <type_traits>
@@ -183,7 +183,8 @@ __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool 
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// 2^((x - ref) log2 e): the difference is formed first, so that what is rounded by the product is as small as it.
+// 2^((x - ref) log2 e): the difference is formed first, so that what is rounded by the product is as small as it. The hardware's
+// exponential serves fp32 as well: 16 ragged sequences of 16 heads of 64 are 1.3e-7 from fp64 with it, the plain fp32 form 1.2e-7.
 __device__ __forceinline__ float exp_from(float x, float ref) { return ex2((x - ref) * kLog2e); }
 
 // Scaled and capped score.
@@ -541,7 +542,8 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) paged_tc_kernel(c
 // A warp step is KS keys, 32 / KS lanes to a key for the scores and DP / 32 columns to a lane for the output; keys and values are
 // staged as fp32. Up to GT query heads share the step. With one head per key-value head the stream bounds it (16 sequences of 16
 // heads of 128: 63 us for a floor of 56; of 64: 22 for 15); with several, the query's and the values' trips through shared memory
-// do, at 8 warps to an SM: 16 sequences with 4 heads to a key-value head of 128 take 55 us for a floor of 28, 16 to one of 80 60 for 9.
+// do, at 8 warps to an SM: 16 sequences with 4 heads to a key-value head of 128 take 55 us for a floor of 28, 16 to one of 80 60 for 9. Operands
+// that are not aligned are loaded element by element, each load waiting where it is issued (16 heads of 64 off the boundary: 350 us, bf16 330).
 template <int DP, int GT> struct SimtShape {
     static constexpr int kKeys = 1024 / DP;                      // 16, 8, 4
     static constexpr int kLanes = 32 / kKeys;                    // lanes per key

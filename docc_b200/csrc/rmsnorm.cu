@@ -3,8 +3,8 @@
 //   s = x + r,  S = round(s),  y = s * rsqrt(mean(s^2) + eps) * gamma,  Y = round(y)  or  Q = e4m3(y / scale_g)
 //
 // Bandwidth bound: x and r are read once, S and Y (or Q and its scales) written once. s stays in fp32 between the sum of
-// squares and the output, so each output is rounded once. Rows of 8192 x 4096 bf16 with residual and 8-bit output: 236 MB, 44.7 us with
-// fresh outputs per call (5.3 TB/s, 0.81 of the measured copy), 38.6 us replayed on the same ones; 8 rows of 1024: 2.0 us.
+// squares and the output, so each output is rounded once. Rows of 8192 x 4096 bf16 with residual and 8-bit output: 236 MB, 45.6 us with
+// fresh outputs per call (5.2 TB/s, 0.79 of the measured copy), 41.4 us replayed on the same ones; 8 rows of 1024: 2.1 us.
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -29,7 +29,8 @@ __device__ __forceinline__ float warp_max_nan(float v) { return __uint_as_float(
 // What turns a group's values into codes: q = e4m3(y / scale), scale = max|y| / 448. The quotient is divided out only where it decides:
 // y times the rounded reciprocal of the scale is off by 2^-23 of the value at most and the rounded quotient by 2^-24, so where both
 // ends of +-2^-21 around that product have the same code, the quotient has it, too. Some 15 values in a million lie nearer to the middle
-// between two codes. The second conversion costs 0.7 us of 45 at 8192 x 4096 and 0.4 of 10.5 at 1021 x 5003; a division per value, 10 us of 54.
+// between two codes. The second conversion costs 0.7 us of 41 at 8192 x 4096 and 0.6 of 10.6 at 1021 x 5003;
+// a division per value cost 10 of 54.
 // A scale that rounded to 0 gives codes of 0. One below fp32's smallest normal number may have no finite reciprocal: the ends 0 and NaN
 // never agree. A scale of inf has the reciprocal 0, a NaN makes every code a NaN.
 __device__ __noinline__ uint32_t quotient_codes(float a, float b, float scale) {  // rare, so a call: the row kernel's loops stay short
@@ -88,7 +89,7 @@ struct RmsArgs {
 };
 
 // Rows whose operands are aligned for 16-byte accesses: TPR threads to a row, which stays in registers (VPT packs each). Eight blocks of
-// 128 threads to an SM (64 registers instead of 72) take the 8192 x 4096 case from 42.2 to 38.6 us, nine or ten spill.
+// 128 threads to an SM (64 registers instead of 72) took the 8192 x 4096 case from 42.2 to 38.6 us, nine or ten spill.
 template <typename T, bool Q8, int TPR, int VPT>
 __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR == 128 ? 8 : 1) rmsnorm_kernel(const T* X, const T* R, T* S, T* Y, uint8_t* Q, float* scales,
                                                                        RmsArgs a) {
@@ -204,8 +205,9 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR == 128 ? 8 : 1) rms
     }
 }
 
-// Any width and alignment: one block per row, the row staged in shared memory, loops that stay loops. Bound by instructions (40 per
-// element with an 8-bit output): 1021 rows of 5003 take 9.8 us, a quarter of the copy rate. The same in registers, unrolled over 20
+// Any width and alignment: one block per row, the row staged in shared memory, loops that stay loops. Bound by the instructions of
+// these loops (one element per load, conversion and store, two more walks through shared memory), not by anything in the data: 1021 rows of
+// 5003 with an 8-bit output take 10.6 us, 1.4 TB/s. The same in registers, unrolled over 20
 // columns per thread, has half as many instructions and took 19.8 us: they no longer fit the instruction cache. On the 16-byte packs
 // of the whole matrix, gamma moved into place by selects, it took 10.8.
 // TPR threads to a row: a block, or a warp.
