@@ -123,13 +123,32 @@ PyObject* tuple_of(std::initializer_list<Tensor> ts) {
 Tensor empty(c10::IntArrayRef shape, const Tensor& like, at::ScalarType type) { return at::empty(shape, like.options().dtype(type).requires_grad(false)); }
 Tensor empty_like(const Tensor& t) { return empty(t.sizes(), t, t.scalar_type()); }
 
-// The entry with the interpreter's lock given up: it may wait, for a stream when its scratch grows or for room in a launch queue. Its
-// arguments have been taken from the tensors before, and the tensors live as long as the caller's arguments.
-template <typename F, typename... Args> int unlocked(F entry, Args... args) {
+// The memory of a call's arguments, kept while the interpreter's lock is given up: another thread may give a tensor other memory then
+// (resize_, set_), and what it had must not be handed out before the kernel that reads it is queued.
+class Held {
+    c10::SmallVector<c10::Storage, 9> storages;
+
+public:
+    Held(std::initializer_list<const Tensor*> tensors) {
+        for (const Tensor* t : tensors)
+            if (t) storages.push_back(t->storage());
+    }
+    template <size_t N> Held(const Tensor* const (&tensors)[N], const Tensor* more) {
+        for (const Tensor* t : tensors) storages.push_back(t->storage());
+        if (more) storages.push_back(more->storage());
+    }
+};
+class Unlocked {
     PyThreadState* const thread = PyEval_SaveThread();
-    const int status = entry(args...);
-    PyEval_RestoreThread(thread);
-    return status;
+
+public:
+    ~Unlocked() { PyEval_RestoreThread(thread); }
+};
+// The entry with the interpreter's lock given up: it may wait, for a stream when its scratch grows or for room in a launch queue. Its
+// arguments have been taken from the tensors before.
+template <typename F, typename... Args> int unlocked(const Held&, F entry, Args... args) {
+    const Unlocked lock;
+    return entry(args...);
 }
 // The answer to a status other than OK.
 PyObject* refused(int status, const char* name) {
@@ -157,6 +176,7 @@ PyObject* norm(PyObject* const* args, Py_ssize_t n, bool quant) {
     if (g && !vector_of(*g, at::kFloat, cols)) Py_RETURN_NONE;
     if (r && (r->scalar_type() != x->scalar_type() || r->sizes() != x->sizes() || !rows_of(*r, rr, rc, ldr))) Py_RETURN_NONE;
     if (quant && (!whole(args[4], group) || (group != 0 && group != 128))) Py_RETURN_NONE;
+    const Held held{x, g, r};
     Tensor s;
     if (r) s = empty_like(*x);
     void* gp = g ? g->data_ptr() : nullptr;
@@ -164,14 +184,14 @@ PyObject* norm(PyObject* const* args, Py_ssize_t n, bool quant) {
     void* sp = r ? s.data_ptr() : nullptr;
     if (!quant) {
         const Tensor y = empty_like(*x);
-        const int status = unlocked(f_rmsnorm, precision(*x), rows, cols, x->data_ptr(), ldx, rp, ldr, gp, eps, sp, y.data_ptr(), 0);
+        const int status = unlocked(held, f_rmsnorm, precision(*x), rows, cols, x->data_ptr(), ldx, rp, ldr, gp, eps, sp, y.data_ptr(), 0);
         if (status != DOCC_B200_OK) return refused(status, "docc_b200_rmsnorm");
         return r ? tuple_of({y, s}) : THPVariable_Wrap(y);
     }
     c10::SmallVector<int64_t, 5> shape(x->sizes().begin(), x->sizes().end());
     shape.back() = group ? (cols + group - 1) / group : 1;
     const Tensor q = empty(x->sizes(), *x, at::kFloat8_e4m3fn), scales = empty(shape, *x, at::kFloat);
-    const int status = unlocked(f_rmsnorm_q8, precision(*x), rows, cols, x->data_ptr(), ldx, rp, ldr, gp, eps, group, sp, q.data_ptr(),
+    const int status = unlocked(held, f_rmsnorm_q8, precision(*x), rows, cols, x->data_ptr(), ldx, rp, ldr, gp, eps, group, sp, q.data_ptr(),
                                 scales.data_ptr(), 0);
     if (status != DOCC_B200_OK) return refused(status, "docc_b200_rmsnorm_q8");
     return r ? tuple_of({q, scales, s}) : tuple_of({q, scales});
@@ -200,9 +220,9 @@ PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const Tensor out = given ? *given : empty_like(*x);
     Strides xs, ys;
     if (!xs.take(*x) || !ys.take(out)) Py_RETURN_NONE;
-    const int status = unlocked(f_rope, precision(*x), x->size(0), x->size(1), x->size(2), 2 * f->size(0), interleaved, inverse, x->data_ptr(), xs.of,
-                                static_cast<const int64_t*>(p->data_ptr()), static_cast<const double*>(f->data_ptr()), float(mscale), out.data_ptr(),
-                                ys.of, 0);
+    const int status = unlocked(Held{x, p, f, given}, f_rope, precision(*x), x->size(0), x->size(1), x->size(2), 2 * f->size(0), interleaved, inverse,
+                                x->data_ptr(), xs.of, static_cast<const int64_t*>(p->data_ptr()), static_cast<const double*>(f->data_ptr()),
+                                float(mscale), out.data_ptr(), ys.of, 0);
     if (status != DOCC_B200_OK) return refused(status, "docc_b200_rope");
     return THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS
@@ -238,10 +258,10 @@ PyObject* rope_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const Tensor out = given ? *given : empty_like(q);
     Strides qs, ks, vs, os, kcs, vcs;
     if (!qs.take(q) || !ks.take(k) || !vs.take(v) || !os.take(out) || !kcs.take(kc) || !vcs.take(vc)) Py_RETURN_NONE;
-    const int status = unlocked(f_rope_append, precision(q), T, q.size(1), kv, D, 2 * f.size(0), interleaved, q.data_ptr(), qs.of, k.data_ptr(),
-                                ks.of, v.data_ptr(), vs.of, static_cast<const int64_t*>(p.data_ptr()), static_cast<const double*>(f.data_ptr()),
-                                float(mscale), out.data_ptr(), os.of, kc.data_ptr(), kcs.of, vc.data_ptr(), vcs.of, kc.size(0), kc.size(2),
-                                static_cast<const int64_t*>(slots.data_ptr()), 0);
+    const int status = unlocked(Held(t, given), f_rope_append, precision(q), T, q.size(1), kv, D, 2 * f.size(0), interleaved, q.data_ptr(), qs.of,
+                                k.data_ptr(), ks.of, v.data_ptr(), vs.of, static_cast<const int64_t*>(p.data_ptr()),
+                                static_cast<const double*>(f.data_ptr()), float(mscale), out.data_ptr(), os.of, kc.data_ptr(), kcs.of, vc.data_ptr(),
+                                vcs.of, kc.size(0), kc.size(2), static_cast<const int64_t*>(slots.data_ptr()), 0);
     if (status != DOCC_B200_OK) return refused(status, "docc_b200_rope_append");
     return THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS
@@ -277,10 +297,11 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Tensor lse;
     if (want_lse) lse = empty({B, Hq}, q, at::kFloat);
     if (args[5] == Py_None) scale = 1.0 / std::sqrt(double(D > 1 ? D : 1));
-    const int status = unlocked(f_paged_attention, precision(q), B, Hq, kv, D, float(scale), float(softcap), window, q.data_ptr(), qs.of,
-                                kc.data_ptr(), kcs.of, vc.data_ptr(), vcs.of, kc.size(0), kc.size(2), static_cast<const int32_t*>(table.data_ptr()),
-                                table.size(1), table.size(1), static_cast<const int32_t*>(lengths.data_ptr()), out.data_ptr(), os.of,
-                                want_lse ? lse.data_ptr() : nullptr, nullptr, 0, 0);
+    const int status = unlocked(Held(t, given), f_paged_attention, precision(q), B, Hq, kv, D, float(scale), float(softcap), window, q.data_ptr(),
+                                qs.of, kc.data_ptr(), kcs.of, vc.data_ptr(), vcs.of, kc.size(0), kc.size(2),
+                                static_cast<const int32_t*>(table.data_ptr()), table.size(1), table.size(1),
+                                static_cast<const int32_t*>(lengths.data_ptr()), out.data_ptr(), os.of, want_lse ? lse.data_ptr() : nullptr, nullptr,
+                                0, 0);
     if (status != DOCC_B200_OK) return refused(status, "docc_b200_paged_attention");
     return want_lse ? tuple_of({out, lse}) : THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS
@@ -299,9 +320,9 @@ PyObject* token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
         Py_RETURN_NONE;
     const Tensor logp = empty({rows}, *x, at::kFloat), entropy = empty({rows}, *x, at::kFloat);
     const Tensor top_ids = empty({rows, k}, *x, at::kLong), top_logp = empty({rows, k}, *x, at::kFloat);
-    const int status = unlocked(f_token_logprobs, precision(*x), rows, vocab, x->data_ptr(), ld, float(scale), static_cast<const
-                                int64_t*>(ids->data_ptr()), logp.data_ptr(), entropy.data_ptr(), k, static_cast<int64_t*>(top_ids.data_ptr()),
-                                top_logp.data_ptr(), 0);
+    const int status = unlocked(Held{x, ids}, f_token_logprobs, precision(*x), rows, vocab, x->data_ptr(), ld, float(scale),
+                                static_cast<const int64_t*>(ids->data_ptr()), logp.data_ptr(), entropy.data_ptr(), k,
+                                static_cast<int64_t*>(top_ids.data_ptr()), top_logp.data_ptr(), 0);
     if (status != DOCC_B200_OK) return refused(status, "docc_b200_token_logprobs");
     return tuple_of({logp, entropy, top_ids, top_logp});
     END_HANDLE_TH_ERRORS

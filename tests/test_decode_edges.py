@@ -428,3 +428,24 @@ def test_calls_on_arrays_of_the_pool(rt, dtype):
         assert same(a, t)
     for a, t in zip(got, want):
         assert isinstance(a, ops.DeviceArray) and np.array_equal(a.to_numpy(), t.cpu().numpy(), equal_nan=a.dtype.kind == "f")
+@gpu
+def test_an_entry_keeps_the_memory_of_its_arguments(rt):
+    """Another thread may run while the entry does. What it takes from an argument meanwhile (here the entry itself does) is not handed
+    out again before the entry has returned."""
+    restype, argtypes = _lib.SIGNATURES["docc_b200_rmsnorm"]
+    x, before, after = torch.zeros(37, 1024, device="cuda"), [], []
+    settle()
+
+    def entry(*args):
+        before.append(x.data_ptr())
+        x.set_()
+        after.append(torch.empty(37, 1024, device="cuda").data_ptr())
+        return 0
+
+    try:
+        stand_in = ctypes.CFUNCTYPE(restype, *argtypes)(entry)
+        bound_to({"docc_b200_rmsnorm": stand_in})
+        ops.rmsnorm(x)
+    finally:
+        bound_to({})
+    assert len(before) == len(after) == 1 and before != after
